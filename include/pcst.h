@@ -33,6 +33,12 @@ extern "C" {
 #define PCST_EINVAL 1001
 #define PCST_EUNSUPPORTED 1002
 
+/* Element types of the block operators (pcst_rms_norm ..., pcst_gated_linear ..., pcst_grad_clip). */
+#define PCST_F32 0
+#define PCST_BF16 1
+#define PCST_F16 2
+#define PCST_E4M3 3 /* OCP 8-bit float, largest value 448 */
+
 /* Library version string, e.g. "pcst 0.1.0 gfx950". */
 const char* pcst_version(void);
 /* Message of the last failing call on this thread ("" if none). */
@@ -485,6 +491,62 @@ int pcst_knn_dist(const float* P, const float* Q, int64_t B, int64_t N, int64_t 
  * (sum over i in order of the nearest unused target's float64 distance) / N.  M <= 262144. */
 int pcst_emd_greedy(const float* P, const float* Q, int64_t B, int64_t N, int64_t M, float* out,
                     void* stream);
+
+/* ---- pre-norm gated residual blocks (models/blocks.py) ------------------------------------ */
+
+/* RMS norm of the rows of x [M,D] (PCST_F32 / BF16 / F16), D <= 16384, with the residual's addition:
+ * s = round(x + residual) (residual may be NULL: s = x and s is not written), rho = 1 / sqrt(mean s^2
+ * + eps), y = s * rho * weight.  weight [D] is of x's type or PCST_F32; y, s [M,D] of x's type;
+ * rho [M] float (may be NULL) is what the backward takes.  Sums and statistics are fp32. */
+int pcst_rms_norm(const void* x, const void* residual, int dtype, int64_t M, int64_t D,
+                  const void* weight, int weight_dtype, float eps, void* y, void* s, float* rho,
+                  void* stream);
+/* The same with an 8-bit output: scale[m] = max |y[m]| / 448 (1 where a row is zero), q = e4m3 of
+ * y / scale, rounded to nearest even. */
+int pcst_rms_norm_quant(const void* x, const void* residual, int dtype, int64_t M, int64_t D,
+                        const void* weight, int weight_dtype, float eps, void* q, float* scale, void* s,
+                        void* stream);
+/* Rows of x [M,D] to e4m3 with a scale for each row (weights of the 8-bit product). */
+int pcst_quant_rows(const void* x, int dtype, int64_t M, int64_t D, void* q, float* scale, void* stream);
+/* Gradients: dx [M,D] (of x and of the residual; the stream's own gradient ds, may be NULL, is added)
+ * and dw [D] (of weight's type); either may be NULL.  s is the forward's stream (x without a
+ * residual).  Deterministic. */
+int pcst_rms_norm_bwd_workspace_size(int64_t M, int64_t D, size_t* bytes);
+int pcst_rms_norm_bwd(const void* s, int dtype, int64_t M, int64_t D, const void* weight,
+                      int weight_dtype, const float* rho, const void* dy, const void* ds, void* dx,
+                      void* dw, void* workspace, void* stream);
+
+/* Gated linear layer: h [M,F] = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel, x [M,D], Wg, Wu [F,D]
+ * of one type, both biases [F] (of that type, or float with bias_f32) or none; act 0 silu, 1 gelu
+ * (erf), 2 relu.  PCST_E4M3 operands carry a scale for each row (x_scale [M], gate_scale, up_scale
+ * [F]) and give out_dtype PCST_BF16 or PCST_F16, their biases are of that or float; elsewhere out_dtype = dtype and the scales are NULL.
+ * Products accumulate in fp32, h is rounded once.  workspace: pcst_gated_linear_workspace_size bytes,
+ * 0 where D * element size is a multiple of 16 and aligned says that x, Wg, Wu start on 16-byte
+ * boundaries (other rows are copied there first). */
+int pcst_gated_linear_workspace_size(int dtype, int64_t M, int64_t D, int64_t F, int aligned, size_t* bytes);
+int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D, const void* w_gate,
+                      const void* w_up, int64_t F, const void* b_gate, const void* b_up, int bias_f32,
+                      int act, const float* x_scale, const float* gate_scale, const float* up_scale,
+                      void* h, int out_dtype, void* workspace, void* stream);
+/* Gradients of the above for dh [M,F] (M > 0; not for e4m3): dx [M,D] of x's type, dw_gate / dw_up
+ * [F,D] of x's type or float (wgrad_f32), db_gate / db_up [F] of the biases' type; each may be NULL.
+ * g and u are recomputed from x, so the forward stores nothing for them.  Deterministic. */
+int pcst_gated_linear_bwd_workspace_size(int dtype, int64_t M, int64_t D, int64_t F, size_t* bytes);
+int pcst_gated_linear_bwd(const void* x, int dtype, int64_t M, int64_t D, const void* w_gate,
+                          const void* w_up, int64_t F, const void* b_gate, const void* b_up, int bias_f32,
+                          int act, const void* dh, void* dx, void* dw_gate, void* dw_up, int wgrad_f32,
+                          void* db_gate, void* db_up, void* workspace, void* stream);
+
+/* Global norm of `count` gradient tensors and clipping (training/trainer.py:118-120):
+ * *norm = |inv_scale| * (sum over all |g|^p)^(1/p), norm_p 1, 2 or 0 (the largest |g|);
+ * out[i] = grads[i] * inv_scale * min(1, max_norm / (*norm + 1e-6)).  grads, out, numel and types are
+ * HOST arrays; types[i] = element type of grads[i] | that of out[i] << 4 (the same, or PCST_F32);
+ * out[i] may be grads[i], and must not overlap another tensor; out NULL: the norm alone.  inv_scale: one float on the device, or
+ * NULL for 1.  A norm that is not finite makes the outputs 0 or NaN, as the formula says. */
+int pcst_grad_clip_workspace_size(const int64_t* numel, int count, size_t* bytes);
+int pcst_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const uint8_t* types,
+                   int count, int norm_p, double max_norm, const float* inv_scale, float* norm,
+                   void* workspace, void* stream);
 
 /* Stream-ordering events with device-scope fences only (hipEventDisableSystemFence; timing = 0
  * also disables timing).  Used by the Python host for the sampling loop's cross-stream

@@ -24,6 +24,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int64
 _D = ctypes.c_double
 _F = ctypes.c_float
+_C = ctypes.c_int
 _SZ = ctypes.POINTER(ctypes.c_size_t)
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
@@ -108,6 +109,18 @@ SIGNATURES = {
     "pcst_l1_workspace_size": [_SZ],
     "pcst_l1_fwd": [_P, _P, _I, _P, _P, _P],
     "pcst_l1_bwd": [_P, _P, _I, _P, _P, _P],
+    "pcst_rms_norm": [_P, _P, _C, _I, _I, _P, _C, _F, _P, _P, _P, _P],
+    "pcst_rms_norm_quant": [_P, _P, _C, _I, _I, _P, _C, _F, _P, _P, _P, _P],
+    "pcst_quant_rows": [_P, _C, _I, _I, _P, _P, _P],
+    "pcst_rms_norm_bwd_workspace_size": [_I, _I, _SZ],
+    "pcst_rms_norm_bwd": [_P, _C, _I, _I, _P, _C, _P, _P, _P, _P, _P, _P, _P],
+    "pcst_gated_linear_workspace_size": [_C, _I, _I, _I, _C, _SZ],
+    "pcst_gated_linear": [_P, _C, _I, _I, _P, _P, _I, _P, _P, _C, _C, _P, _P, _P, _P, _C, _P, _P],
+    "pcst_gated_linear_bwd_workspace_size": [_C, _I, _I, _I, _SZ],
+    "pcst_gated_linear_bwd": [_P, _C, _I, _I, _P, _P, _I, _P, _P, _C, _C, _P, _P, _P, _P, _C, _P, _P, _P,
+                              _P],
+    "pcst_grad_clip_workspace_size": [_P, _C, _SZ],
+    "pcst_grad_clip": [_P, _P, _P, _P, _C, _C, _D, _P, _P, _P, _P],
     "pcst_event_create": [ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)],
     "pcst_event_destroy": [_P],
     "pcst_event_record": [_P, _P],
@@ -1311,6 +1324,274 @@ def voxel_downsample_copies_dseed(points, target, seed_dev, copies):
     return out_pts, out_idx
 
 
+# ----------------------------------------------------------------------------- gated residual blocks
+# element types of the block operators at the C boundary (pcst.h: PCST_F32 ..)
+_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+ACTS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _same_device(what, t, *others):
+    require_device(t, *others)
+    d = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != d:
+            raise RuntimeError(f"{what}: tensors on different devices ({t.device}, {o.device})")
+
+
+def _norm_operands(what, x, weight, residual):
+    """x, weight and residual of a row norm, checked: (x, weight, residual) contiguous, M, D."""
+    if x.dim() < 1 or x.dtype not in _FLOATS:
+        raise RuntimeError(f"{what}: x is a float32, bfloat16 or float16 tensor [..., D], got {x.dtype}")
+    D = x.shape[-1]
+    if D == 0:
+        raise RuntimeError(f"{what}: rows of no values")
+    if weight is not None:
+        if tuple(weight.shape) != (D,) or weight.dtype not in (x.dtype, torch.float32):
+            raise RuntimeError(f"{what}: weight is [{D}] of {x.dtype} or float32, got {weight.dtype} "
+                               f"{list(weight.shape)}")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise RuntimeError(f"{what}: residual is {x.dtype} {list(x.shape)} like x, got "
+                               f"{residual.dtype} {list(residual.shape)}")
+    _same_device(what, x, weight, residual)
+    return (x.contiguous(), None if weight is None else weight.contiguous(),
+            None if residual is None else residual.contiguous(), x.numel() // D, D)
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, stats=False):
+    """s = x + residual (rounded to x's type), y = s / sqrt(mean(s^2) + eps) * weight over the last
+    dimension -> (y, s, rho): s is x itself without a residual, rho [rows] float32 (1 / the root mean
+    square, for rms_norm_bwd) is None unless stats."""
+    x, weight, residual, M, D = _norm_operands("rms_norm", x, weight, residual)
+    y = torch.empty_like(x)
+    s = x if residual is None else torch.empty_like(x)
+    rho = torch.empty(M, dtype=torch.float32, device=x.device) if stats else None
+    _call("pcst_rms_norm", _ptr(x), _ptr(residual), _ELEM[x.dtype], M, D, _ptr(weight),
+          _ELEM[weight.dtype], eps, _ptr(y), _ptr(s), _ptr(rho), _stream())
+    return y, s, rho
+
+
+def rms_norm_bwd(s, weight, rho, dy, ds=None, need_dx=True, need_dw=True):
+    """Gradients of rms_norm: s, rho as it returned them, dy (of y), ds (of s, or None) ->
+    (dx, dw); dx is the gradient of x and of the residual alike.  Deterministic."""
+    s, weight, dy, M, D = _norm_operands("rms_norm_bwd", s, weight, dy)
+    _same_device("rms_norm_bwd", s, rho, ds)
+    if rho.dtype != torch.float32 or rho.numel() != M:
+        raise RuntimeError(f"rms_norm_bwd: rho is float32 [{M}]")
+    if ds is not None:
+        if ds.shape != s.shape or ds.dtype != s.dtype:
+            raise RuntimeError("rms_norm_bwd: ds has s's shape and type")
+        ds = ds.contiguous()
+    rho = rho.contiguous()
+    dx = torch.empty_like(s) if need_dx else None
+    dw = torch.empty_like(weight) if need_dw else None
+    ws = _workspace("pcst_rms_norm_bwd_workspace_size", M, D, device=s.device) if need_dw else None
+    _call("pcst_rms_norm_bwd", _ptr(s), _ELEM[s.dtype], M, D, _ptr(weight), _ELEM[weight.dtype],
+          _ptr(rho), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw), _ptr(ws), _stream())
+    return dx, dw
+
+
+def rms_norm_quant(x, weight, residual=None, eps=1e-6):
+    """rms_norm with an 8-bit output -> (q float8_e4m3fn like x, scale float32 [rows], s):
+    scale = max |y| / 448 over a row (1 for a row of zeros), q = y / scale rounded to nearest even."""
+    x, weight, residual, M, D = _norm_operands("rms_norm_quant", x, weight, residual)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    s = x if residual is None else torch.empty_like(x)
+    _call("pcst_rms_norm_quant", _ptr(x), _ptr(residual), _ELEM[x.dtype], M, D, _ptr(weight),
+          _ELEM[weight.dtype], eps, _ptr(q), _ptr(scale), _ptr(s), _stream())
+    return q, scale, s
+
+
+def quant_rows(x):
+    """x [..., D] -> (q float8_e4m3fn like x, scale float32 [...]): rows in 8 bits, as
+    rms_norm_quant's."""
+    x, _, _, M, D = _norm_operands("quant_rows", x, None, None)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call("pcst_quant_rows", _ptr(x), _ELEM[x.dtype], M, D, _ptr(q), _ptr(scale), _stream())
+    return q, scale
+
+
+def _gated_operands(what, x, w_gate, w_up, b_gate, b_up, act, bias_dtype):
+    if act not in ACTS:
+        raise RuntimeError(f"{what}: act is one of {sorted(ACTS)}, got {act!r}")
+    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[1]:
+        raise RuntimeError(f"{what}: shapes are x [M,D], w_gate and w_up [F,D], got {list(x.shape)}, "
+                           f"{list(w_gate.shape)}, {list(w_up.shape)}")
+    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise RuntimeError(f"{what}: x and the weights are of one type, got {x.dtype}, {w_gate.dtype}, "
+                           f"{w_up.dtype}")
+    if (b_gate is None) != (b_up is None):
+        raise RuntimeError(f"{what}: both biases or none")
+    F = w_gate.shape[0]
+    if b_gate is not None:
+        if tuple(b_gate.shape) != (F,) or tuple(b_up.shape) != (F,) or b_gate.dtype != b_up.dtype \
+                or b_gate.dtype not in (bias_dtype, torch.float32):
+            raise RuntimeError(f"{what}: the biases are [{F}] of {bias_dtype} or float32")
+    if F == 0 or x.shape[1] == 0:
+        raise RuntimeError(f"{what}: no features ({list(x.shape)}, {list(w_gate.shape)})")
+    _same_device(what, x, w_gate, w_up, b_gate, b_up)
+    if b_gate is not None:
+        b_gate, b_up = b_gate.contiguous(), b_up.contiguous()
+    return x.contiguous(), w_gate.contiguous(), w_up.contiguous(), b_gate, b_up
+
+
+def _bias_f32(b):
+    return 1 if b is not None and b.dtype == torch.float32 else 0
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=None, out_dtype=None):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up): x [M,D], weights [F,D] of one type (float32,
+    bfloat16, float16), biases [F] of that type or float32 -> [M,F] of that type, products in fp32,
+    rounded once.  act: "silu", "gelu" (erf) or "relu".  float8_e4m3fn operands take scales = (x's
+    [M], w_gate's [F], w_up's [F]) and out_dtype, bfloat16 or float16."""
+    out_dtype = out_dtype or x.dtype
+    e4m3 = x.dtype == torch.float8_e4m3fn
+    if x.dtype not in _ELEM or out_dtype not in _FLOATS or (not e4m3 and out_dtype != x.dtype):
+        raise RuntimeError(f"gated_linear: no product of {x.dtype} operands into {out_dtype}")
+    if e4m3 and out_dtype == torch.float32:
+        raise RuntimeError("gated_linear: float8_e4m3fn operands give bfloat16 or float16")
+    if (scales is not None) != e4m3 or (e4m3 and len(scales) != 3):
+        raise RuntimeError("gated_linear: float8_e4m3fn operands take scales (x, w_gate, w_up), others none")
+    x, w_gate, w_up, b_gate, b_up = _gated_operands("gated_linear", x, w_gate, w_up, b_gate, b_up, act,
+                                                    out_dtype)
+    M, D = x.shape
+    F = w_gate.shape[0]
+    xs = gs = us = None
+    if e4m3:
+        for t, n in zip(scales, (M, F, F)):
+            if t.dtype != torch.float32 or t.numel() != n:
+                raise RuntimeError("gated_linear: scales are float32, one for each row")
+        _same_device("gated_linear", x, *scales)
+        xs, gs, us = (t.contiguous() for t in scales)
+    h = torch.empty(M, F, dtype=out_dtype, device=x.device)
+    dt = _ELEM[x.dtype]
+    ws = None
+    aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
+    if not aligned or D * x.element_size() % 16:
+        ws = _workspace("pcst_gated_linear_workspace_size", dt, M, D, F, int(aligned), device=x.device)
+    _call("pcst_gated_linear", _ptr(x), dt, M, D, _ptr(w_gate), _ptr(w_up), F, _ptr(b_gate), _ptr(b_up),
+          _bias_f32(b_gate), ACTS[act], _ptr(xs), _ptr(gs), _ptr(us), _ptr(h), _ELEM[out_dtype], _ptr(ws),
+          _stream())
+    return h
+
+
+def gated_linear_bwd(x, w_gate, w_up, dh, b_gate=None, b_up=None, act="silu", need=(True,) * 5,
+                     wgrad_dtype=None):
+    """Gradients of gated_linear for dh [M,F]: need = which of (dx, dw_gate, dw_up, db_gate, db_up) ->
+    these five (None where not needed, and for absent biases).  dw in wgrad_dtype: x's type (default)
+    or float32; db in the biases' type.  Deterministic."""
+    wgrad_dtype = wgrad_dtype or x.dtype
+    if x.dtype not in _FLOATS or wgrad_dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"gated_linear_bwd: no gradients of {x.dtype} operands in {wgrad_dtype}")
+    x, w_gate, w_up, b_gate, b_up = _gated_operands("gated_linear_bwd", x, w_gate, w_up, b_gate, b_up, act,
+                                                    x.dtype)
+    M, D = x.shape
+    F = w_gate.shape[0]
+    if tuple(dh.shape) != (M, F) or dh.dtype != x.dtype:
+        raise RuntimeError(f"gated_linear_bwd: dh is {x.dtype} [{M},{F}], got {dh.dtype} {list(dh.shape)}")
+    _same_device("gated_linear_bwd", x, dh)
+    dh = dh.contiguous()
+    dev = x.device
+    new = torch.zeros if M == 0 else torch.empty
+    dx = torch.empty_like(x) if need[0] else None
+    dw = [new(F, D, dtype=wgrad_dtype, device=dev) if n else None for n in need[1:3]]
+    db = [new(F, dtype=b_gate.dtype, device=dev) if n and b_gate is not None else None for n in need[3:5]]
+    if M and any(t is not None for t in [dx, *dw, *db]):
+        dt = _ELEM[x.dtype]
+        ws = _workspace("pcst_gated_linear_bwd_workspace_size", dt, M, D, F, device=dev)
+        _call("pcst_gated_linear_bwd", _ptr(x), dt, M, D, _ptr(w_gate), _ptr(w_up), F, _ptr(b_gate),
+              _ptr(b_up), _bias_f32(b_gate), ACTS[act], _ptr(dh), _ptr(dx), _ptr(dw[0]), _ptr(dw[1]),
+              1 if wgrad_dtype == torch.float32 else 0, _ptr(db[0]), _ptr(db[1]), _ptr(ws), _stream())
+    return (dx, *dw, *db)
+
+
+# ----------------------------------------------------------------------------- gradient clipping
+def _dense(t):
+    """Whether t's elements fill its memory without gaps, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for size, stride in sorted(((a, b) for a, b in zip(t.shape, t.stride()) if a != 1), key=lambda p: p[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+_NORM_P = {1.0: 1, 2.0: 2, float("inf"): 0}
+
+
+def grad_clip(grads, max_norm, norm_type=2.0, inv_scale=None, out=None, scale=True):
+    """The norm of all `grads` together (times inv_scale, a float32 device tensor of one element) ->
+    float32 tensor []; with scale, out[i] = grads[i] * inv_scale * min(1, max_norm / (norm + 1e-6)),
+    out None: in place.  grads: dense tensors of float32, bfloat16 or float16 on one device, no two of
+    them (or of the outputs) overlapping; out[i] like grads[i] in shape and strides, of its type or
+    float32.  norm_type 1, 2 or inf.  Nothing waits for the device."""
+    grads = list(grads)
+    p = _NORM_P.get(float(norm_type))
+    if p is None:
+        raise RuntimeError(f"grad_clip: norm_type is 1, 2 or inf, got {norm_type}")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise RuntimeError(f"grad_clip: max_norm is at least 0, got {max_norm}")
+    n = len(grads)
+    if n == 0:
+        raise RuntimeError("grad_clip: no gradients")
+    if out is not None:
+        out = list(out)
+        if len(out) != n:
+            raise RuntimeError(f"grad_clip: {len(out)} outputs for {n} gradients")
+    dev = grads[0].get_device()
+    for t in grads if out is None else grads + out:
+        if t.dtype not in _FLOATS or t.layout != torch.strided:
+            raise RuntimeError(f"grad_clip: dense float32, bfloat16 or float16 tensors only, got {t.dtype} "
+                               f"({t.layout})")
+        if not (t.is_contiguous() or _dense(t)):
+            raise RuntimeError(f"grad_clip: a tensor with gaps (strides {t.stride()} of {list(t.shape)}); "
+                               "pass its contiguous copy")
+    ptr = np.fromiter([t.data_ptr() for t in grads], np.int64, n)
+    numel = np.fromiter([t.numel() for t in grads], np.int64, n)
+    elem = np.fromiter([_ELEM[t.dtype] for t in grads], np.uint8, n)
+    lo, hi = ptr, ptr + numel * np.where(elem == 0, 4, 2)
+    optr, oelem = ptr, elem
+    if out is not None:
+        for g, o in zip(grads, out):
+            if o.shape != g.shape or not (o.dtype == g.dtype or o.dtype == torch.float32) \
+                    or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                raise RuntimeError("grad_clip: an output has its gradient's shape and strides, and its type "
+                                   f"or float32; got {o.dtype} {list(o.shape)} for {g.dtype} {list(g.shape)}")
+        optr = np.fromiter([t.data_ptr() for t in out], np.int64, n)
+        oelem = np.fromiter([_ELEM[t.dtype] for t in out], np.uint8, n)
+        other = (optr != ptr) | (oelem != elem)
+        lo = np.concatenate([lo, optr[other]])
+        hi = np.concatenate([hi, (optr + numel * np.where(oelem == 0, 4, 2))[other]])
+    some = hi > lo
+    lo, hi = lo[some], hi[some]
+    order = np.argsort(lo)
+    if bool((lo[order][1:] < hi[order][:-1]).any()):
+        raise RuntimeError("grad_clip: two of the tensors overlap (or one is given twice)")
+    if inv_scale is not None and (inv_scale.dtype != torch.float32 or inv_scale.numel() != 1
+                                  or inv_scale.get_device() != dev):
+        raise RuntimeError("grad_clip: inv_scale is one float32 on the gradients' device")
+    if dev < 0 or any(t.get_device() != dev for t in (grads if out is None else grads + out)):
+        require_device(*grads)
+        raise RuntimeError("grad_clip: tensors on different devices")
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    types = elem | (oelem << 4)
+    sz = ctypes.c_size_t(0)
+    np_ptr = lambda a: ctypes.c_void_p(a.ctypes.data)  # noqa: E731
+    _call("pcst_grad_clip_workspace_size", np_ptr(numel), n, ctypes.byref(sz))
+    ws = torch.empty(sz.value, dtype=torch.uint8, device=norm.device)
+    _call("pcst_grad_clip", np_ptr(ptr), np_ptr(optr) if scale else None, np_ptr(numel), np_ptr(types), n, p,
+          max_norm, _ptr(inv_scale), _ptr(norm), _ptr(ws), _stream())
+    if scale:  # what autograd saved of these tensors is now another value
+        torch.autograd.graph.increment_version(grads if out is None else out)
+    return norm
+
+
 # every public wrapper launches on its tensors' device (see _on_tensor_device)
 _GUARDED = ("square_distance", "index_points", "fps", "ball_query", "group_gather",
             "voxel_downsample", "voxel_stats", "knn3_build", "knn3_query", "knn3_interp",
@@ -1321,7 +1602,9 @@ _GUARDED = ("square_distance", "index_points", "fps", "ball_query", "group_gathe
             "bn_relu_maxpool", "bn_relu_bwd", "group_gather_bwd", "group_colsum16", "resblock_fwd16", "resblock_bwd16", "cast16_batch",
             "gemm_ex", "dropout_grad_bf16",
             "linear_wgrad_ex", "knn_workspace", "voxel_copies_workspace", "knn3_rows_build",
-            "knn3_rows_refs", "knn3_rows_query", "knn_rows_stats", "knn3_interp_rows")
+            "knn3_rows_refs", "knn3_rows_query", "knn_rows_stats", "knn3_interp_rows",
+            "rms_norm", "rms_norm_bwd", "rms_norm_quant", "quant_rows", "gated_linear", "gated_linear_bwd",
+            "grad_clip")
 for _name in _GUARDED:
     globals()[_name] = _on_tensor_device(globals()[_name])
 del _name

@@ -1,0 +1,707 @@
+// The matrix products of the gated linear layer (gated_linear.hip), for one operand type per
+// translation unit.
+//
+//   forward     h[m, f] = act(g) * u,   g = sum_d x[m, d] Wg[f, d] + bg[f],   u likewise with Wu, bu
+//   backward    dg = dh * u * act'(g),  du = dh * act(g)       (g and u recomputed, stored as [dg | du])
+//               dx[m, d] = sum_f dg[m, f] Wg[f, d] + du[m, f] Wu[f, d]
+//               dW[f, d] = sum_m dg[m, f] x[m, d]              (Wg; du for Wu)
+//
+// One tiled product serves all: out[m, n] = sum_k A(m, k) B(n, k), where either operand lies with k
+// contiguous (x, W in the forward; [dg | du] in dx) or with its row index contiguous (W in dx; both
+// operands of dW).  A work-group owns BM rows and two column blocks of BNH: Wg's and Wu's rows of the
+// same features in the forward (so a lane holds g and u of the same element and the activation and the
+// product need no exchange), neighbouring columns elsewhere.
+//
+// Staging: 128 bytes of k a stage (64 16-bit values, 32 floats, 128 e4m3), two stages, loaded from
+// global memory straight into LDS while the other stage is multiplied.  The LDS image is linear in the
+// order of the loading lanes; each lane picks the 16-byte piece it fetches (an XOR of the piece's index
+// with bits of its row), so that the 16-byte fragment reads -- and the transposed 8-byte reads of
+// operands whose rows are contiguous -- spread over the banks.  Loads past a tile's rows or past k are
+// sent past the buffer's end and arrive as zeros, so ragged sizes take no other path.
+//
+// The MFMA takes B's rows as its row operand, so a lane's four accumulators are four consecutive output
+// columns; with k contiguous, the rows of a wave's tiles are dealt so that a lane's tiles follow each
+// other as well: 4 * TNH consecutive outputs a lane, whole lines a wave, and no pass through LDS.
+#pragma once
+#include "ops_types.h"
+
+namespace pcst {
+namespace gated {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+#define PCST_LDS __attribute__((address_space(3)))
+
+enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
+enum { EPI_FWD = 0, EPI_BWD = 1, EPI_OUT = 2 };
+
+constexpr int kRowB = 128;  // bytes of k per stage
+
+struct GemmArgs {
+  const char* a[2];   // row operand, per k segment
+  const char* b0[2];  // column operand, per k segment: first (or only) matrix
+  const char* b1[2];  // second matrix (forward / recompute)
+  int64_t lda, ldb;   // bytes
+  int64_t M;          // rows (per group)
+  int N;              // columns of a column block's matrix
+  int64_t K;          // per segment
+  int nseg;
+  int tiles_m, tiles_n, ntiles, per_xcd;
+  int splits;         // of k (row-contiguous operands only)
+  int64_t kps;        // k per split
+  int groups;         // independent products of one launch (dWg, dWu): group g's A starts a_group bytes on
+  int64_t a_group, o_group, o_split;  // bytes, elements, elements
+  void* out;
+  int64_t ldo;        // elements
+  const void *bg, *bu;
+  int bias_f32, act;
+  const void* dh;
+  int64_t fpad;       // backward: du starts at column fpad of the [dg | du] rows
+  float* bpart;       // backward: bias partials [row block, 2, N] or null
+  const float *xs, *gs, *us;  // e4m3 scales
+};
+
+__device__ __forceinline__ rsrc_t make_rsrc(const char* p, int64_t bytes) {
+  const int n = bytes <= 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, n, 0x00020000);
+}
+
+template <class E>
+constexpr int elem_size() {
+  return (int)sizeof(typename E::T);
+}
+
+// D += A B over the 16 bytes of k that a lane of each operand holds
+template <class E>
+__device__ __forceinline__ f32x4 mma16(i32x4 a, i32x4 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mma16<EBF16>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<EF16>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<EF32>(i32x4 a, i32x4 b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
+  return c;
+}
+// e4m3: 32 bytes a lane, one 16x16x128 product (unit block scales); which k a byte is, is the same
+// for both operands, which is all that the sum over k needs.  The unit adds the products of 8 bytes at 14
+// bits below the binade of the largest (measured) and these sums in fp32: enough for a 16-bit result
+// (2^-9 and 2^-11), not for a float one, so the 8-bit form has no float output.
+__device__ __forceinline__ f32x4 mma32_e4m3(i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1, f32x4 c) {
+  const i32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+  const i32x8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+}
+
+// ---- activations: the 16-bit types take the hardware's exp2 and reciprocal (1 ulp of fp32 each, far
+// below a 16-bit rounding); fp32 the accurate functions
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float g) {
+  if (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
+  return 1.0f / (1.0f + expf(-g));
+}
+template <bool FAST>
+__device__ __forceinline__ float act_value(float g, int act) {
+  if (act == ACT_SILU) return g * sigmoid<FAST>(g);
+  if (act == ACT_GELU) return g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
+  return g > 0.0f ? g : g * 0.0f;  // NaN stays NaN
+}
+template <bool FAST>
+__device__ __forceinline__ float act_grad(float g, int act, float& value) {
+  if (act == ACT_SILU) {
+    const float e = sigmoid<FAST>(g);
+    value = g * e;
+    return e * (1.0f + g * (1.0f - e));
+  }
+  if (act == ACT_GELU) {
+    const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    value = g * c;
+    return c + g * expf(-0.5f * g * g) * 0.3989422804014327f;
+  }
+  value = g > 0.0f ? g : g * 0.0f;
+  return g > 0.0f ? 1.0f : g * 0.0f;
+}
+
+// ---- LDS images.  KC: row r holds 128 bytes of k; piece c of 16 bytes at position c ^ swz(r).
+// Row operand: 16 lanes read rows 16 i + 0..15 -> swz = (r >> 1) & 7.
+// Column operand: 16 lanes read rows (l >> 2) * 4 TNH + (l & 3) -> bits 1 and log2(4 TNH), + 1.
+template <int TNH, bool COL>
+__device__ __forceinline__ int swz_kc(int r) {
+  if (!COL) return (r >> 1) & 7;
+  constexpr int S = TNH == 4 ? 4 : 3;
+  return ((r >> 1) & 1) | (((r >> S) & 3) << 1);
+}
+// MN: row k holds W elements; 16-bit: transposed reads of rows k..k+3 (a group of 16 lanes) at 32
+// bytes; fp32: 16 lanes read 64 bytes of one row, the four groups rows 4 apart
+template <int ES, int CPR>
+__device__ __forceinline__ int swz_mn(int k) {
+  if (ES == 2) return (2 * ((k & 3) | (((k >> 3) & 1) << 2))) & (CPR - 1);
+  return (4 * ((k >> 2) & 3)) & (CPR - 1);
+}
+
+// One operand's image of R rows (KC) or R columns (MN): R * 128 bytes either way
+template <class E, bool MN, bool COL, int R, int TNH, int NW>
+struct Stage {
+  static constexpr int ES = elem_size<E>();
+  static constexpr int RB = R * ES;          // MN: bytes of one k row
+  static constexpr int CPR = RB / 16;
+  static constexpr int IT = R / 8 / NW;      // 1 KiB loads per wave
+  static_assert(R % (8 * NW) == 0, "whole loads per wave");
+  uint32_t off[IT];
+  int piece[IT];  // KC: byte offset of the piece in its row (for the end of k)
+
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) {
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+      const int at = (wave + NW * j) * 1024 + lane * 16;
+      if (MN) {
+        const int k = at / RB, p = (at % RB) / 16;
+        off[j] = (uint32_t)(k * ld + ((p ^ swz_mn<ES, CPR>(k)) * 16));
+        piece[j] = 0;
+      } else {
+        const int r = at / kRowB, p = (at % kRowB) / 16;
+        piece[j] = (p ^ swz_kc<TNH, COL>(r)) * 16;
+        off[j] = (uint32_t)(r * ld + piece[j]);
+      }
+    }
+  }
+  // base: the tile's first byte at this stage's first k; bytes: up to the end of what may be read;
+  // kleft: bytes of k left (KC)
+  __device__ __forceinline__ void load(PCST_LDS char* img, const char* base, int64_t bytes, int kleft, int wave) const {
+    const rsrc_t r = make_rsrc(base, bytes);
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+      const uint32_t o = MN || piece[j] < kleft ? off[j] : 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (PCST_LDS void*)(img + (wave + NW * j) * 1024), 16, (int)o, 0, 0, 0);
+    }
+  }
+};
+
+// Fragment reads of one wave: T tiles of 16 rows from row r0 on (COL: dealt as 4 T consecutive rows a
+// lane group); a lane gets 16 bytes of k of step ks
+template <class E, bool MN, bool COL, int R, int T, int TNH>
+struct Frag {
+  static constexpr int ES = elem_size<E>();
+  static constexpr int RB = R * ES, CPR = RB / 16;
+  int at[MN ? T : 2];
+
+  __device__ __forceinline__ void init(int r0, int lane) {
+    const int l = lane & 15, g = lane >> 4;
+    if (MN) {
+#pragma unroll
+      for (int t = 0; t < (MN ? T : 2); ++t) {
+        if (ES == 2) {
+          const int q = l >> 2, p = l & 3, k = 8 * g + q;
+          const int c = (r0 + 16 * t) / 8 + (p >> 1);
+          at[t] = k * RB + ((c ^ swz_mn<ES, CPR>(k)) * 16) + (p & 1) * 8;
+        } else {
+          const int k = 4 * g, c = (r0 + 16 * t) / 4 + (l >> 2);
+          at[t] = k * RB + ((c ^ swz_mn<ES, CPR>(k)) * 16) + (l & 3) * 4;
+        }
+      }
+    } else {
+      const int r = r0 + (COL ? (l >> 2) * 4 * TNH + (l & 3) : l);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) at[ks] = r * kRowB + (((ks * 4 + g) ^ swz_kc<TNH, COL>(r)) * 16);
+    }
+  }
+  __device__ __forceinline__ i32x4 read(const PCST_LDS char* img, int t, int ks) const {
+    if (MN) {
+      i32x4 v;
+      if (ES == 2) {
+        const PCST_LDS char* p = img + at[MN ? t : 0] + ks * 32 * RB;
+        const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((PCST_LDS i16x4*)p));
+        const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((PCST_LDS i16x4*)(p + 4 * RB)));
+        v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = *(const PCST_LDS int*)(img + at[MN ? t : 0] + (ks * 16 + j) * RB);
+      }
+      return v;
+    }
+    return *(const PCST_LDS i32x4*)(img + at[MN ? 0 : ks] + t * (COL ? 4 : 16) * kRowB);
+  }
+};
+
+// 4 consecutive outputs, the first n of them
+template <class O>
+__device__ __forceinline__ void store4(O* p, int n, f32x4 v) {
+  struct __attribute__((packed, aligned(sizeof(O)))) V4 { O v[4]; };
+  if (n >= 4) {
+    V4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.v[i] = (O)v[i];
+    *reinterpret_cast<V4*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = (O)v[i];
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void load_bias8(const void* b, int f32, int f, int n, float (&v)[8]) {
+  if (!b || n <= 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  } else if (f32) {
+    load8(static_cast<const float*>(b) + f, n, v);
+  } else {
+    load8(static_cast<const T*>(b) + f, n, v);
+  }
+}
+
+// E: operand type, O: output type, NMN / MMN: the column / row operand's row index is contiguous
+template <class E, class O, bool NMN, bool MMN, int EPI, int BM, int BNH, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
+  constexpr int NW = WM * WN, TM = BM / WM / 16, TNH = BNH / WN / 16;
+  constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
+  constexpr bool GATED = EPI != EPI_OUT;
+  constexpr bool FAST = ES < 4;
+  static_assert(!GATED || !NMN, "the forward reads W with k contiguous");
+  // one array per stage and operand, so that the compiler sees which loads a read has to wait for
+  __shared__ __attribute__((aligned(1024))) char lds_a0[BM * kRowB], lds_a1[BM * kRowB];
+  __shared__ __attribute__((aligned(1024))) char lds_b0[2 * BNH * kRowB], lds_b1[2 * BNH * kRowB];
+
+  // work-group L runs on XCD L % 8; an XCD's tiles follow each other in blocks of 4 row tiles, so that
+  // what its work-groups read at a time is shared in its L2
+  const int L = blockIdx.x;
+  int t = (L & 7) * g.per_xcd + (L >> 3);
+  if (t >= g.ntiles) return;
+  const int tiles_mn = g.tiles_m * g.tiles_n;
+  const int gs_ = t / tiles_mn;
+  t -= gs_ * tiles_mn;
+  const int group = gs_ % g.groups, split = gs_ / g.groups;
+  const int band = t / (4 * g.tiles_n), inb = t - band * 4 * g.tiles_n;
+  const int bh = g.tiles_m - 4 * band < 4 ? g.tiles_m - 4 * band : 4;
+  const int tm = 4 * band + inb % bh, tn = inb / bh;
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * (GATED ? BNH : 2 * BNH);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  Stage<E, MMN, false, BM, TNH, NW> sa;
+  Stage<E, NMN, true, NMN ? 2 * BNH : BNH, TNH, NW> sb;
+  sa.init(wave, lane, g.lda);
+  sb.init(wave, lane, g.ldb);
+  Frag<E, MMN, false, BM, TM, TNH> fa;
+  Frag<E, NMN, true, NMN ? 2 * BNH : BNH, TNH, TNH> fb[NMN ? 2 : 1];
+  fa.init(wm * 16 * TM, lane);
+  fb[0].init(wn * 16 * TNH, lane);
+  if (NMN) fb[NMN ? 1 : 0].init(BNH + wn * 16 * TNH, lane);
+
+  f32x4 acc[2][TNH][TM];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < TNH; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int64_t kb = (int64_t)split * g.kps;
+  const int64_t klen = kb + g.kps < g.K ? g.kps : g.K - kb;
+  const int nk = (int)((klen + BKE - 1) / BKE), total = nk * g.nseg;
+
+  auto load = [&](int it, PCST_LDS char* ia, PCST_LDS char* ib) {
+    const int seg = it >= nk ? 1 : 0;
+    const int64_t k = (int64_t)(it - seg * nk) * BKE;
+    const char* a = g.a[seg] + group * g.a_group;
+    if (MMN)
+      sa.load(ia, a + (kb + k) * g.lda + m0 * ES, (klen - k) * g.lda - m0 * ES, 0, wave);
+    else
+      sa.load(ia, a + m0 * g.lda + (kb + k) * ES, (g.M - m0 < BM ? g.M - m0 : BM) * g.lda - (kb + k) * ES,
+              (int)((klen - k) * ES < kRowB ? (klen - k) * ES : kRowB), wave);
+    if (NMN) {
+      sb.load(ib, g.b0[seg] + (kb + k) * g.ldb + (int64_t)n0 * ES, (klen - k) * g.ldb - (int64_t)n0 * ES, 0, wave);
+    } else {
+      const int kl = (int)((klen - k) * ES < kRowB ? (klen - k) * ES : kRowB);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int nh = GATED ? n0 : n0 + h * BNH;
+        const char* b = GATED && h ? g.b1[seg] : g.b0[seg];
+        const int rows = g.N - nh < BNH ? g.N - nh : BNH;
+        sb.load(ib + h * BNH * kRowB, b + (int64_t)nh * g.ldb + (kb + k) * ES,
+                rows <= 0 ? 0 : (int64_t)rows * g.ldb - (kb + k) * ES, kl, wave);
+      }
+    }
+  };
+
+  auto compute = [&](const PCST_LDS char* ia, const PCST_LDS char* ib) {
+    if constexpr (ES == 1) {
+      i32x4 a[2][TM];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) a[ks][i] = fa.read(ia, i, ks);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TNH; ++j) {
+          const i32x4 b0 = fb[0].read(ib + h * BNH * kRowB, j, 0), b1 = fb[0].read(ib + h * BNH * kRowB, j, 1);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma32_e4m3(b0, b1, a[0][i], a[1][i], acc[h][j][i]);
+        }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4 a[TM], b[2][TNH];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) a[i] = fa.read(ia, i, ks);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < TNH; ++j)
+            b[h][j] = NMN ? fb[NMN ? h : 0].read(ib, j, ks) : fb[0].read(ib + h * BNH * kRowB, j, ks);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < TNH; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) acc[h][j][i] = mma16<E>(b[h][j], a[i], acc[h][j][i]);
+      }
+    }
+  };
+
+  PCST_LDS char* a0 = (PCST_LDS char*)lds_a0;
+  PCST_LDS char* a1 = (PCST_LDS char*)lds_a1;
+  PCST_LDS char* b0 = (PCST_LDS char*)lds_b0;
+  PCST_LDS char* b1 = (PCST_LDS char*)lds_b1;
+  if (total > 0) load(0, a0, b0);
+  for (int it = 0; it < total; it += 2) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this stage's loads, this wave's
+    __syncthreads();                                  // everyone's; and the other stage has been read
+    if (it + 1 < total) load(it + 1, a1, b1);
+    compute(a0, b0);
+    if (it + 1 >= total) break;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (it + 2 < total) load(it + 2, a0, b0);
+    compute(a1, b1);
+  }
+
+  // ---- epilogue
+  const int l = lane & 15, q = lane >> 4;
+  if constexpr (GATED) {
+    constexpr int RUN = 4 * TNH;  // consecutive features of a lane
+    const int f0 = n0 + wn * 16 * TNH + q * RUN;
+    const int nf = g.N - f0;
+    float csum[2][RUN];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < RUN; ++k) csum[h][k] = 0.0f;
+#pragma unroll
+    for (int p = 0; p < RUN / 8; ++p) {
+      const int f = f0 + 8 * p, n = nf - 8 * p;
+      float bg[8], bu[8], sg[8], su[8];
+      load_bias8<O>(g.bg, g.bias_f32, f, n, bg);
+      load_bias8<O>(g.bu, g.bias_f32, f, n, bu);
+      if (ES == 1) {
+        load_bias8<float>(g.gs, 1, f, n, sg);
+        load_bias8<float>(g.us, 1, f, n, su);
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + wm * 16 * TM + 16 * i + l;
+        float gv[8], uv[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          gv[k] = acc[0][2 * p + k / 4][i][k % 4];
+          uv[k] = acc[1][2 * p + k / 4][i][k % 4];
+        }
+        if (ES == 1) {
+          const float xs = m < g.M ? g.xs[m] : 0.0f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            gv[k] *= xs * sg[k];
+            uv[k] *= xs * su[k];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          gv[k] += bg[k];
+          uv[k] += bu[k];
+        }
+        if (EPI == EPI_FWD) {
+          if (m < g.M && n > 0) {
+            float o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = act_value<FAST>(gv[k], g.act) * uv[k];
+            store8(static_cast<O*>(g.out) + m * g.ldo + f, n, o);
+          }
+        } else if (m < g.M && f < g.fpad) {
+          float d[8], og[8], ou[8];
+          if (n > 0) {
+            load8(static_cast<const O*>(g.dh) + m * g.N + f, n, d);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[k] = 0.0f;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float v;
+            const float da = act_grad<FAST>(gv[k], g.act, v);
+            og[k] = k < n ? d[k] * uv[k] * da : 0.0f;  // the padding up to fpad is zero
+            ou[k] = k < n ? d[k] * v : 0.0f;
+            csum[0][8 * p + k] += og[k];
+            csum[1][8 * p + k] += ou[k];
+          }
+          O* o = static_cast<O*>(g.out) + m * g.ldo + f;
+          store8(o, 8, og);
+          store8(o + g.fpad, 8, ou);
+        }
+      }
+    }
+    if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
+      float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+          float v = csum[h][k];
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+          if (l == 0 && k < nf) bp[(int64_t)h * g.N + f0 + k] = v;
+        }
+    }
+  } else {
+    O* out = static_cast<O*>(g.out) + group * g.o_group + split * g.o_split;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + wm * 16 * TM + 16 * i + l;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TNH; ++j) {
+          const int n = n0 + h * BNH + wn * 16 * TNH + (NMN ? 16 * j + 4 * q : q * 4 * TNH + 4 * j);
+          if (n < g.N) store4(out + m * g.ldo + n, g.N - n, acc[h][j][i]);
+        }
+    }
+  }
+}
+
+// ---- host side of one operand type
+struct FwdCall {
+  const void *x, *wg, *wu;
+  int64_t M, D, F, ldx, ldw;  // pitches in bytes, 16-byte multiples, bases 16-byte aligned
+  const void *bg, *bu;
+  int bias_f32, act, out_type;
+  const float *xs, *gs, *us;
+  void* h;
+};
+struct BwdCall {
+  FwdCall f;
+  const void* dh;
+  void* dgu;       // [M, 2 * fpad]
+  int64_t fpad;
+  float *bpart, *wpart;
+  void *dx, *dwg, *dwu, *dbg, *dbu;
+  int wgrad_f32, bgrad_f32;
+};
+
+constexpr int kBigTiles = 200;  // launches of at least this many large tiles take them
+
+inline bool take_big(int64_t M, int64_t N, int nw) { return cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
+
+struct WgradPlan {
+  bool big;
+  int splits;
+  int64_t kps;
+};
+// dW's tiles are few and its k is long: split k until about 512 work-groups run, at least 8 stages each
+inline WgradPlan wgrad_plan(int64_t M, int64_t D, int64_t F, int es) {
+  WgradPlan p;
+  p.big = 2 * cdiv(F, 256) * cdiv(D, 256) >= kBigTiles;
+  const int64_t tiles = p.big ? 2 * cdiv(F, 256) * cdiv(D, 256) : 2 * cdiv(F, 128) * cdiv(D, 128);
+  const int64_t bke = kRowB / es;
+  int64_t s = std::max<int64_t>(1, 512 / tiles);
+  s = std::max<int64_t>(1, std::min<int64_t>(s, cdiv(M, 8 * bke)));
+  p.kps = cdiv(cdiv(M, s), bke) * bke;
+  p.splits = (int)std::max<int64_t>(1, cdiv(M, p.kps));
+  return p;
+}
+inline int64_t bias_parts(int64_t M, int64_t F) { return take_big(M, F, 128) ? cdiv(M, 256) * 4 : cdiv(M, 128) * 2; }
+
+template <class E>
+int fwd(const FwdCall& c, void* stream);
+template <class E>
+int bwd(const BwdCall& c, void* stream);
+
+#ifdef PCST_GATED_IMPL
+template <class E, class O, bool NMN, bool MMN, int EPI, bool BIG>
+int launch(GemmArgs& g, hipStream_t s) {
+  constexpr int BM = BIG ? 256 : 128, BNH = BIG ? 128 : 64, WM = BIG ? 4 : 2, WN = 2;
+  constexpr int NT = EPI == EPI_OUT ? 2 * BNH : BNH;
+  const int64_t tm = cdiv(g.M, BM), tn = cdiv(g.N, NT), n = tm * tn * g.groups * g.splits;
+  PCST_CHECK_ARG(n < (1ll << 30), "gated_linear: too many tiles");
+  g.tiles_m = (int)tm;
+  g.tiles_n = (int)tn;
+  g.ntiles = (int)n;
+  g.per_xcd = (int)cdiv(n, 8);
+  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, BM, BNH, WM, WN>), dim3((unsigned)(g.per_xcd * 8)),
+                     dim3(64 * WM * WN), 0, s, g);
+  PCST_LAUNCH_CHECK("gated_linear");
+  return PCST_OK;
+}
+
+inline GemmArgs fwd_args(const FwdCall& c) {
+  GemmArgs g{};
+  g.a[0] = static_cast<const char*>(c.x);
+  g.b0[0] = static_cast<const char*>(c.wg);
+  g.b1[0] = static_cast<const char*>(c.wu);
+  g.lda = c.ldx;
+  g.ldb = c.ldw;
+  g.M = c.M;
+  g.N = (int)c.F;
+  g.K = g.kps = c.D;
+  g.nseg = g.splits = g.groups = 1;
+  g.bg = c.bg;
+  g.bu = c.bu;
+  g.bias_f32 = c.bias_f32;
+  g.act = c.act;
+  g.xs = c.xs;
+  g.gs = c.gs;
+  g.us = c.us;
+  return g;
+}
+
+template <class E, class O>
+int fwd_out(const FwdCall& c, hipStream_t s) {
+  GemmArgs g = fwd_args(c);
+  g.out = c.h;
+  g.ldo = c.F;
+  return take_big(c.M, c.F, 128) ? launch<E, O, false, false, EPI_FWD, true>(g, s)
+                                 : launch<E, O, false, false, EPI_FWD, false>(g, s);
+}
+
+// dW's partials (a split's lie `stride` after the previous one's) added in order
+template <class O>
+__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, int64_t n, int64_t stride,
+                                                      int parts, O* __restrict__ out) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * stride + e];
+  out[e] = (O)s;
+}
+// 16 columns a work-group, 16 slices of the parts
+template <class O>
+__global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ part, int F, int parts, O* dbg, O* dbu) {
+  __shared__ double red[16][17];
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int f = blockIdx.x * 16 + c;  // of 2 F
+  double s = 0.0;
+  if (f < 2 * F) {
+#pragma unroll 8
+    for (int p = q; p < parts; p += 16) s += (double)part[(int64_t)p * 2 * F + f];
+  }
+  red[q][c] = s;
+  __syncthreads();
+  if (q == 0 && f < 2 * F) {
+    for (int i = 1; i < 16; ++i) s += red[i][c];
+    O* o = f < F ? dbg : dbu;
+    if (o) o[f < F ? f : f - F] = (O)(float)s;
+  }
+}
+
+template <class E>
+int bwd_impl(const BwdCall& c, hipStream_t s) {
+  typedef typename E::T T;
+  constexpr int ES = elem_size<E>();
+  const FwdCall& f = c.f;
+  GemmArgs g = fwd_args(f);
+  g.out = c.dgu;
+  g.ldo = 2 * c.fpad;
+  g.fpad = c.fpad;
+  g.dh = c.dh;
+  g.bpart = c.dbg || c.dbu ? c.bpart : nullptr;
+  int rc = take_big(f.M, f.F, 128) ? launch<E, T, false, false, EPI_BWD, true>(g, s)
+                                   : launch<E, T, false, false, EPI_BWD, false>(g, s);
+  if (rc) return rc;
+  if (g.bpart) {
+    const dim3 grid((unsigned)cdiv(2 * f.F, 16));
+    const int parts = (int)bias_parts(f.M, f.F);
+    if (c.bgrad_f32)
+      hipLaunchKernelGGL(bias_kernel<float>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts,
+                         static_cast<float*>(c.dbg), static_cast<float*>(c.dbu));
+    else
+      hipLaunchKernelGGL(bias_kernel<T>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts, static_cast<T*>(c.dbg),
+                         static_cast<T*>(c.dbu));
+    PCST_LAUNCH_CHECK("gated_linear_bwd");
+  }
+  if (c.dx) {
+    GemmArgs d{};
+    d.a[0] = static_cast<const char*>(c.dgu);
+    d.a[1] = d.a[0] + c.fpad * ES;
+    d.b0[0] = static_cast<const char*>(f.wg);
+    d.b0[1] = static_cast<const char*>(f.wu);
+    d.lda = 2 * c.fpad * ES;
+    d.ldb = f.ldw;
+    d.M = f.M;
+    d.N = (int)f.D;
+    d.K = d.kps = f.F;
+    d.nseg = 2;
+    d.splits = d.groups = 1;
+    d.out = c.dx;
+    d.ldo = f.D;
+    rc = take_big(f.M, f.D, 256) ? launch<E, T, true, false, EPI_OUT, true>(d, s)
+                                 : launch<E, T, true, false, EPI_OUT, false>(d, s);
+    if (rc) return rc;
+  }
+  if (c.dwg || c.dwu) {
+    const WgradPlan p = wgrad_plan(f.M, f.D, f.F, ES);
+    GemmArgs w{};
+    w.a[0] = static_cast<const char*>(c.dgu);
+    w.b0[0] = static_cast<const char*>(f.x);
+    w.lda = 2 * c.fpad * ES;
+    w.ldb = f.ldx;
+    w.M = f.F;
+    w.N = (int)f.D;
+    w.K = f.M;
+    w.kps = p.kps;
+    w.nseg = 1;
+    w.splits = p.splits;
+    w.groups = 2;
+    w.a_group = c.fpad * ES;
+    w.ldo = f.D;
+    w.out = c.wpart;
+    w.o_group = f.F * f.D;
+    w.o_split = 2 * f.F * f.D;
+    rc = p.big ? launch<E, float, true, true, EPI_OUT, true>(w, s) : launch<E, float, true, true, EPI_OUT, false>(w, s);
+    if (rc) return rc;
+    const int64_t n = f.F * f.D;
+    const dim3 grid((unsigned)cdiv(n, 256));
+    for (int k = 0; k < 2; ++k) {
+      void* o = k ? c.dwu : c.dwg;
+      if (!o) continue;
+      if (c.wgrad_f32)
+        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, s, c.wpart + k * n, n, 2 * n, p.splits,
+                           static_cast<float*>(o));
+      else
+        hipLaunchKernelGGL(combine_kernel<T>, grid, dim3(256), 0, s, c.wpart + k * n, n, 2 * n, p.splits,
+                           static_cast<T*>(o));
+    }
+    PCST_LAUNCH_CHECK("gated_linear_bwd");
+  }
+  return PCST_OK;
+}
+#endif  // PCST_GATED_IMPL
+
+}  // namespace gated
+}  // namespace pcst

@@ -1,0 +1,231 @@
+// The global norm of many gradient tensors, and clipping by it.
+//
+//   N = inv * (sum over all tensors of |g|^p)^(1/p),  p = 1, 2 or inf
+//   c = min(1, max_norm / (N + 1e-6)) * inv,          out = g * c
+//
+// Two launches (per 128 tensors): the norm's, whose work-groups each leave one partial in fp64, and
+// the scaling's, whose work-groups each add all partials in the same fixed order themselves -- at most
+// 1024 + (number of tensors) of them, so that no third launch, no atomic and no zeroed counter stands
+// between.  fp64 sums: a square of any finite float is finite there, and the order does not show in the
+// 24 bits returned.  The tensors' addresses travel in the kernel arguments, so a captured launch keeps
+// them.  Bound by HBM: every gradient is read twice and written once.
+#include "ops_types.h"
+
+namespace pcst {
+namespace {
+
+constexpr int kClipTensors = 128;  // per launch: 128 * 29 bytes of kernel arguments
+
+struct ClipTable {
+  const void* in[kClipTensors];
+  void* out[kClipTensors];
+  int64_t n[kClipTensors];
+  int32_t first[kClipTensors + 1];  // a tensor's first chunk
+  uint8_t type[kClipTensors];       // element type code, the output's in the high half
+  int32_t count;
+};
+
+// chunk of this work-group -> (tensor, element range)
+__device__ __forceinline__ int find_tensor(const ClipTable& t, int chunk) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// the larger one, NaN where either is one
+__device__ __forceinline__ double nan_max(double a, double b) { return (b > a || b != b) ? b : a; }
+
+__device__ __forceinline__ double wave_total(double v, int p) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const double t = __shfl_xor(v, o, 64);
+    v = p == 0 ? nan_max(v, t) : v + t;
+  }
+  return v;
+}
+
+// all 256 threads' values together, in the same order on every thread
+__device__ __forceinline__ double block_total(double v, int p, double* red) {
+  v = wave_total(v, p);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = red[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = p == 0 ? nan_max(s, red[i]) : s + red[i];
+  return s;
+}
+
+template <class T>
+__device__ __forceinline__ double range_sum(const T* g, int64_t lo, int64_t hi, int p) {
+  double s = 0.0;
+#pragma unroll 2
+  for (int64_t i = lo + threadIdx.x * 8; i < hi; i += 256 * 8) {
+    float v[8];
+    load8(g + i, (int)(hi - i < 8 ? hi - i : 8), v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double d = (double)v[j];
+      s = p == 2 ? fma(d, d, s) : p == 1 ? s + fabs(d) : nan_max(s, fabs(d));
+    }
+  }
+  return s;
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(ClipTable t, int64_t chunk_len, int p,
+                                                        double* __restrict__ part) {
+  __shared__ double red[4];
+  const int k = find_tensor(t, blockIdx.x);
+  const int64_t lo = (int64_t)(blockIdx.x - t.first[k]) * chunk_len;
+  const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
+  const int type = t.type[k] & 15;
+  double s;
+  if (type == kF32) s = range_sum(static_cast<const float*>(t.in[k]), lo, hi, p);
+  else if (type == kBF16) s = range_sum(static_cast<const __bf16*>(t.in[k]), lo, hi, p);
+  else s = range_sum(static_cast<const _Float16*>(t.in[k]), lo, hi, p);
+  s = block_total(s, p, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+template <class T, class O>
+__device__ __forceinline__ void range_scale(const T* g, O* o, int64_t lo, int64_t hi, float f) {
+#pragma unroll 2
+  for (int64_t i = lo + threadIdx.x * 8; i < hi; i += 256 * 8) {
+    const int n = (int)(hi - i < 8 ? hi - i : 8);
+    float v[8];
+    load8(g + i, n, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    store8(o + i, n, v);
+  }
+}
+
+__global__ __launch_bounds__(256) void grad_scale_kernel(ClipTable t, int64_t chunk_len, int p,
+                                                         const double* __restrict__ part, int parts,
+                                                         double max_norm, const float* inv_scale,
+                                                         float* __restrict__ norm) {
+  __shared__ double red[4];
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < parts; i += 256) s = p == 0 ? nan_max(s, part[i]) : s + part[i];
+  s = block_total(s, p, red);
+  const double inv = inv_scale ? (double)*inv_scale : 1.0;
+  const double total = (p == 2 ? sqrt(s) : s) * fabs(inv);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+  double c = max_norm / (total + 1e-6);
+  c = c > 1.0 ? 1.0 : c;  // NaN stays
+  const float f = (float)(c * inv);
+  const int k = find_tensor(t, blockIdx.x);
+  if (f == 1.0f && t.in[k] == t.out[k]) return;  // g * 1 is g
+  const int64_t lo = (int64_t)(blockIdx.x - t.first[k]) * chunk_len;
+  const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
+  const void* g = t.in[k];
+  void* o = t.out[k];
+  switch (t.type[k]) {
+    case kF32 | kF32 << 4: range_scale(static_cast<const float*>(g), static_cast<float*>(o), lo, hi, f); break;
+    case kBF16 | kBF16 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<__bf16*>(o), lo, hi, f); break;
+    case kF16 | kF16 << 4: range_scale(static_cast<const _Float16*>(g), static_cast<_Float16*>(o), lo, hi, f); break;
+    case kBF16 | kF32 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<float*>(o), lo, hi, f); break;
+    default: range_scale(static_cast<const _Float16*>(g), static_cast<float*>(o), lo, hi, f); break;
+  }
+}
+
+// elements per work-group: about 1024 work-groups over all tensors, at least 2048 elements each
+int64_t clip_chunk(int64_t total) { return std::max<int64_t>(2048, cdiv(cdiv(total, 1024), 2048) * 2048); }
+
+int64_t clip_total(const int64_t* n, int count) {
+  int64_t t = 0;
+  for (int i = 0; i < count; ++i) t += n[i];
+  return t;
+}
+
+int64_t clip_parts(const int64_t* n, int count, int64_t chunk) {
+  int64_t t = 0;
+  for (int i = 0; i < count; ++i) t += cdiv(n[i], chunk);
+  return t;
+}
+
+template <class F>
+void for_tables(const void* const* in, void* const* out, const int64_t* n, const uint8_t* type, int count,
+                int64_t chunk, F f) {
+  int64_t base = 0;
+  for (int i = 0; i < count;) {
+    ClipTable t;
+    t.count = 0;
+    int32_t c = 0;
+    for (; i < count && t.count < kClipTensors; ++i) {
+      if (n[i] == 0) continue;
+      t.in[t.count] = in[i];
+      t.out[t.count] = out ? out[i] : nullptr;
+      t.n[t.count] = n[i];
+      t.type[t.count] = type[i];
+      t.first[t.count++] = c;
+      c += (int32_t)cdiv(n[i], chunk);
+    }
+    if (t.count == 0) break;
+    t.first[t.count] = c;
+    f(t, c, base);
+    base += c;
+  }
+}
+
+// the norm alone (no outputs)
+__global__ __launch_bounds__(256) void grad_total_kernel(const double* __restrict__ part, int parts, int p,
+                                                         const float* inv_scale, float* __restrict__ norm) {
+  __shared__ double red[4];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) s = p == 0 ? nan_max(s, part[i]) : s + part[i];
+  s = block_total(s, p, red);
+  if (threadIdx.x == 0) *norm = (float)((p == 2 ? sqrt(s) : s) * fabs(inv_scale ? (double)*inv_scale : 1.0));
+}
+
+bool is_float(int t) { return t == kF32 || t == kBF16 || t == kF16; }
+
+}  // namespace
+}  // namespace pcst
+
+using namespace pcst;
+
+extern "C" int pcst_grad_clip_workspace_size(const int64_t* numel, int count, size_t* bytes) {
+  PCST_CHECK_ARG(count >= 0 && (count == 0 || numel) && bytes, "grad_clip_workspace_size: bad args");
+  *bytes = sizeof(double) * (size_t)std::max<int64_t>(1, clip_parts(numel, count, clip_chunk(clip_total(numel, count))));
+  return PCST_OK;
+}
+
+extern "C" int pcst_grad_clip(const void* const* grads, void* const* out, const int64_t* numel,
+                              const uint8_t* types, int count, int norm_p, double max_norm,
+                              const float* inv_scale, float* norm, void* workspace, void* stream) {
+  PCST_CHECK_ARG(count >= 0 && (count == 0 || (grads && numel && types)) && norm, "grad_clip: null pointer");
+  PCST_CHECK_ARG(norm_p >= 0 && norm_p <= 2, "grad_clip: norm_p is 1, 2 or 0 (the largest absolute value)");
+  PCST_CHECK_ARG(max_norm >= 0, "grad_clip: max_norm is at least 0");
+  for (int i = 0; i < count; ++i) {
+    const int ti = types[i] & 15, to = types[i] >> 4;
+    PCST_CHECK_ARG(is_float(ti) && (to == ti || to == kF32),
+                   "grad_clip: tensor %d: gradients are float32, bfloat16 or float16, outputs of their type or float32", i);
+    PCST_CHECK_ARG(numel[i] >= 0 && (numel[i] == 0 || (grads[i] && (!out || out[i]))),
+                   "grad_clip: tensor %d: bad size or null pointer", i);
+  }
+  const int64_t total = clip_total(numel, count);
+  PCST_CHECK_ARG(total < (1ll << 40), "grad_clip: too many elements");
+  hipStream_t s = as_stream(stream);
+  PCST_CHECK_ARG(total == 0 || workspace, "grad_clip: null workspace");
+  double* part = static_cast<double*>(workspace);
+  const int64_t chunk = clip_chunk(total);
+  const int parts = (int)clip_parts(numel, count, chunk);
+  for_tables(grads, out, numel, types, count, chunk, [&](const ClipTable& t, int32_t c, int64_t base) {
+    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)c), dim3(256), 0, s, t, chunk, norm_p, part + base);
+  });
+  if (!out || parts == 0) {
+    hipLaunchKernelGGL(grad_total_kernel, dim3(1), dim3(256), 0, s, part, parts, norm_p, inv_scale, norm);
+    PCST_LAUNCH_CHECK("grad_clip");
+    return PCST_OK;
+  }
+  for_tables(grads, out, numel, types, count, chunk, [&](const ClipTable& t, int32_t c, int64_t base) {
+    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)c), dim3(256), 0, s, t, chunk, norm_p, part, parts,
+                       max_norm, inv_scale, base ? nullptr : norm);
+  });
+  PCST_LAUNCH_CHECK("grad_clip");
+  return PCST_OK;
+}

@@ -7,6 +7,15 @@ from .diffusion_model import (
     PointCloudDiffusionModel,
     DiffusionProcess,
 )
+from .blocks import (
+    GatedLinear,
+    RMSNorm,
+    gated_linear,
+    gated_linear_quant,
+    quant_rows,
+    rms_norm,
+    rms_norm_quant,
+)
 from .losses import DiffusionLoss
 from .pointnet2_encoder import PointNet2Encoder
 
@@ -19,4 +28,11 @@ __all__ = [
     "DiffusionProcess",
     "DiffusionLoss",
     "PointNet2Encoder",
+    "RMSNorm",
+    "GatedLinear",
+    "rms_norm",
+    "rms_norm_quant",
+    "quant_rows",
+    "gated_linear",
+    "gated_linear_quant",
 ]

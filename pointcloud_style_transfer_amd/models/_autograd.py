@@ -21,6 +21,7 @@ The SetAbstraction training half (csrc/sa_train.hip):
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _hip
 
@@ -423,6 +424,65 @@ class GroupGatherFn(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dp = _hip.group_gather_bwd(g_grouped, group_idx, ctx.N)
         return None, dp, None, None
+
+
+class RMSNormFn(torch.autograd.Function):
+    """(y, s) of _hip.rms_norm: s = x + residual is the next block's stream, y the norm of it."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s, rho = _hip.rms_norm(x, weight, residual, eps, stats=True)
+        ctx.save_for_backward(s, weight, rho)
+        ctx.set_materialize_grads(False)
+        if residual is None:
+            return y
+        return y, s
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight, rho = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:  # only the stream went on
+            return ds if need_x else None, None, ds if need_r else None, None
+        dx, dw = _hip.rms_norm_bwd(s, weight, rho, dy, ds, need_x or need_r, need_w)
+        return dx if need_x else None, dw, dx if need_r else None, None
+
+
+class GatedLinearFn(torch.autograd.Function):
+    """_hip.gated_linear with its gradients; under autocast the operands are rounded to its 16-bit type
+    and the gradients of float32 weights are float32.  g and u are recomputed in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
+        shape = x.shape
+        x2 = x.reshape(-1, shape[-1])
+        half = autocast_half() if x.is_cuda else None
+        ctx.types = (x.dtype, w_gate.dtype, w_up.dtype)
+        wg, wu = w_gate.detach(), w_up.detach()
+        if half is not None:
+            x2 = x2.to(half)
+            if wg.dtype == wu.dtype == torch.float32:
+                wg, wu = _cast_all([wg, wu], half)
+            else:
+                wg, wu = wg.to(half), wu.to(half)
+            b_gate, b_up = (b if b is None or b.dtype in (half, torch.float32) else b.to(half)
+                            for b in (b_gate, b_up))
+        h = _hip.gated_linear(x2, wg, wu, b_gate, b_up, act)
+        ctx.save_for_backward(x2, wg, wu, b_gate, b_up)
+        ctx.act, ctx.shape = act, shape
+        return h.view(*shape[:-1], h.shape[-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x2, wg, wu, b_gate, b_up = ctx.saved_tensors
+        f32 = ctx.types[1] == ctx.types[2] == torch.float32
+        dx, dwg, dwu, dbg, dbu = _hip.gated_linear_bwd(
+            x2, wg, wu, dh.reshape(-1, wg.shape[0]).to(x2.dtype), b_gate, b_up, ctx.act,
+            ctx.needs_input_grad[:5], torch.float32 if f32 else None)
+        dx = None if dx is None else dx.to(ctx.types[0]).view(ctx.shape)
+        return dx, dwg, dwu, dbg, dbu, None
 
 
 def linear(x, lin, relu=False):
