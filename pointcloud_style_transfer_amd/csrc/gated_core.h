@@ -60,7 +60,7 @@ struct GemmArgs {
   void* out;
   int64_t ldo;        // elements
   const void *bg, *bu;
-  int bias_f32, act;
+  int bias_f32;
   const void* dh;
   int64_t fpad;       // backward: du starts at column fpad of the [dg | du] rows
   float* bpart;       // backward: bias partials [row block, 2, N] or null
@@ -112,23 +112,35 @@ __device__ __forceinline__ float sigmoid(float g) {
   if (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
   return 1.0f / (1.0f + expf(-g));
 }
+// 1 + erf(g / sqrt 2), e = exp(-g^2 / 2): Abramowitz and Stegun 7.1.26 (1.5e-7 absolute) for the 16-bit types
 template <bool FAST>
-__device__ __forceinline__ float act_value(float g, int act) {
-  if (act == ACT_SILU) return g * sigmoid<FAST>(g);
-  if (act == ACT_GELU) return g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
-  return g > 0.0f ? g : g * 0.0f;  // NaN stays NaN
+__device__ __forceinline__ float gelu_cdf2(float g, float e) {
+  if (!FAST) return 1.0f + erff(g * 0.70710678118654752f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.3275911f * 0.70710678118654752f, 1.0f));
+  const float c = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  return g < 0.0f ? c * e : 2.0f - c * e;
 }
 template <bool FAST>
-__device__ __forceinline__ float act_grad(float g, int act, float& value) {
-  if (act == ACT_SILU) {
+__device__ __forceinline__ float gauss(float g) {
+  return FAST ? __builtin_amdgcn_exp2f(g * g * -0.72134752044448170f) : expf(-0.5f * g * g);
+}
+template <bool FAST, int ACT>
+__device__ __forceinline__ float act_value(float g) {
+  if (ACT == ACT_SILU) return g * sigmoid<FAST>(g);
+  if (ACT == ACT_GELU) return 0.5f * g * gelu_cdf2<FAST>(g, FAST ? gauss<true>(g) : 0.0f);
+  return g > 0.0f ? g : g * 0.0f;  // NaN stays NaN
+}
+template <bool FAST, int ACT>
+__device__ __forceinline__ float act_grad(float g, float& value) {
+  if (ACT == ACT_SILU) {
     const float e = sigmoid<FAST>(g);
     value = g * e;
     return e * (1.0f + g * (1.0f - e));
   }
-  if (act == ACT_GELU) {
-    const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+  if (ACT == ACT_GELU) {
+    const float e = gauss<FAST>(g), c = 0.5f * gelu_cdf2<FAST>(g, e);
     value = g * c;
-    return c + g * expf(-0.5f * g * g) * 0.3989422804014327f;
+    return fmaf(g * e, 0.3989422804014327f, c);
   }
   value = g > 0.0f ? g : g * 0.0f;
   return g > 0.0f ? 1.0f : g * 0.0f;
@@ -264,7 +276,7 @@ __device__ __forceinline__ void load_bias8(const void* b, int f32, int f, int n,
 }
 
 // E: operand type, O: output type, NMN / MMN: the column / row operand's row index is contiguous
-template <class E, class O, bool NMN, bool MMN, int EPI, int BM, int BNH, int WM, int WN>
+template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, int BM, int BNH, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TNH = BNH / WN / 16;
   constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
@@ -317,13 +329,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   const int nk = (int)((klen + BKE - 1) / BKE), total = nk * g.nseg;
 
   auto load = [&](int it, PCST_LDS char* ia, PCST_LDS char* ib) {
-    const int seg = it >= nk ? 1 : 0;
-    const int64_t k = (int64_t)(it - seg * nk) * BKE;
+    const int seg = it >= nk && g.nseg > 1 ? 1 : 0;
+    const int64_t k = (int64_t)(it - seg * nk) * BKE;  // past klen: no bytes left
     const char* a = g.a[seg] + group * g.a_group;
     if (MMN)
       sa.load(ia, a + (kb + k) * g.lda + m0 * ES, (klen - k) * g.lda - m0 * ES, 0, wave);
     else
-      sa.load(ia, a + m0 * g.lda + (kb + k) * ES, (g.M - m0 < BM ? g.M - m0 : BM) * g.lda - (kb + k) * ES,
+      sa.load(ia, a + m0 * g.lda + (kb + k) * ES, k < klen ? (g.M - m0 < BM ? g.M - m0 : BM) * g.lda - (kb + k) * ES : 0,
               (int)((klen - k) * ES < kRowB ? (klen - k) * ES : kRowB), wave);
     if (NMN) {
       sb.load(ib, g.b0[seg] + (kb + k) * g.ldb + (int64_t)n0 * ES, (klen - k) * g.ldb - (int64_t)n0 * ES, 0, wave);
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
         const char* b = GATED && h ? g.b1[seg] : g.b0[seg];
         const int rows = g.N - nh < BNH ? g.N - nh : BNH;
         sb.load(ib + h * BNH * kRowB, b + (int64_t)nh * g.ldb + (kb + k) * ES,
-                rows <= 0 ? 0 : (int64_t)rows * g.ldb - (kb + k) * ES, kl, wave);
+                rows <= 0 || k >= klen ? 0 : (int64_t)rows * g.ldb - (kb + k) * ES, kl, wave);
       }
     }
   };
@@ -356,23 +368,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           for (int i = 0; i < TM; ++i) acc[h][j][i] = mma32_e4m3(b0, b1, a[0][i], a[1][i], acc[h][j][i]);
         }
     } else {
+      // four groups (k step, column block) of TM * TNH products; a group's products run while the next
+      // one's fragments are read
+      i32x4 a[2][TM], b[2][TNH];
+      auto read_a = [&](int ks) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x4 a[TM], b[2][TNH];
+        for (int i = 0; i < TM; ++i) a[ks][i] = fa.read(ia, i, ks);
+      };
+      auto read_b = [&](int ks, int h) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[i] = fa.read(ia, i, ks);
+        for (int j = 0; j < TNH; ++j)
+          b[h][j] = NMN ? fb[NMN ? h : 0].read(ib, j, ks) : fb[0].read(ib + h * BNH * kRowB, j, ks);
+      };
+      auto mma = [&](int ks, int h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < TNH; ++j)
 #pragma unroll
-          for (int j = 0; j < TNH; ++j)
-            b[h][j] = NMN ? fb[NMN ? h : 0].read(ib, j, ks) : fb[0].read(ib + h * BNH * kRowB, j, ks);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < TNH; ++j)
-#pragma unroll
-            for (int i = 0; i < TM; ++i) acc[h][j][i] = mma16<E>(b[h][j], a[i], acc[h][j][i]);
-      }
+          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma16<E>(b[h][j], a[ks][i], acc[h][j][i]);
+      };
+      read_a(0);
+      read_b(0, 0);
+      read_b(0, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      mma(0, 0);
+      read_a(1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_b(1, 0);
+      mma(0, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_b(1, 1);
+      mma(1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      mma(1, 1);
     }
   };
 
@@ -380,18 +407,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   PCST_LDS char* a1 = (PCST_LDS char*)lds_a1;
   PCST_LDS char* b0 = (PCST_LDS char*)lds_b0;
   PCST_LDS char* b1 = (PCST_LDS char*)lds_b1;
-  if (total > 0) load(0, a0, b0);
-  for (int it = 0; it < total; it += 2) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this stage's loads, this wave's
+  // pairs of stages in one basic block (the accumulators stay in place); a load past the last stage
+  // fetches nothing
+  auto next = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the stage
     __syncthreads();                                  // everyone's; and the other stage has been read
-    if (it + 1 < total) load(it + 1, a1, b1);
+  };
+  load(0, a0, b0);
+  for (int it = 0; it + 2 <= total; it += 2) {
+    next();
+    load(it + 1, a1, b1);
     compute(a0, b0);
-    if (it + 1 >= total) break;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (it + 2 < total) load(it + 2, a0, b0);
+    next();
+    load(it + 2, a0, b0);
     compute(a1, b1);
   }
+  next();
+  if (total & 1) compute(a0, b0);
 
   // ---- epilogue
   const int l = lane & 15, q = lane >> 4;
@@ -399,15 +431,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     constexpr int RUN = 4 * TNH;  // consecutive features of a lane
     const int f0 = n0 + wn * 16 * TNH + q * RUN;
     const int nf = g.N - f0;
-    float csum[2][RUN];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < RUN; ++k) csum[h][k] = 0.0f;
 #pragma unroll
     for (int p = 0; p < RUN / 8; ++p) {
       const int f = f0 + 8 * p, n = nf - 8 * p;
-      float bg[8], bu[8], sg[8], su[8];
+      float bg[8], bu[8], sg[8], su[8], csum[2][8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) csum[0][k] = csum[1][k] = 0.0f;
       load_bias8<O>(g.bg, g.bias_f32, f, n, bg);
       load_bias8<O>(g.bu, g.bias_f32, f, n, bu);
       if (ES == 1) {
@@ -440,7 +469,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
           if (m < g.M && n > 0) {
             float o[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = act_value<FAST>(gv[k], g.act) * uv[k];
+            for (int k = 0; k < 8; ++k) o[k] = act_value<FAST, ACT>(gv[k]) * uv[k];
             store8(static_cast<O*>(g.out) + m * g.ldo + f, n, o);
           }
         } else if (m < g.M && f < g.fpad) {
@@ -454,29 +483,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             float v;
-            const float da = act_grad<FAST>(gv[k], g.act, v);
+            const float da = act_grad<FAST, ACT>(gv[k], v);
             og[k] = k < n ? d[k] * uv[k] * da : 0.0f;  // the padding up to fpad is zero
             ou[k] = k < n ? d[k] * v : 0.0f;
-            csum[0][8 * p + k] += og[k];
-            csum[1][8 * p + k] += ou[k];
+            csum[0][k] += og[k];
+            csum[1][k] += ou[k];
           }
           O* o = static_cast<O*>(g.out) + m * g.ldo + f;
           store8(o, 8, og);
           store8(o + g.fpad, 8, ou);
         }
       }
-    }
-    if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
-      float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N;
+      if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
+        float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N + f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < RUN; ++k) {
-          float v = csum[h][k];
+          for (int k = 0; k < 8; ++k) {
+            float v = csum[h][k];
 #pragma unroll
-          for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-          if (l == 0 && k < nf) bp[(int64_t)h * g.N + f0 + k] = v;
-        }
+            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+            if (l == 0 && k < n) bp[(int64_t)h * g.N + k] = v;
+          }
+      }
     }
   } else {
     O* out = static_cast<O*>(g.out) + group * g.o_group + split * g.o_split;
@@ -543,7 +572,7 @@ template <class E>
 int bwd(const BwdCall& c, void* stream);
 
 #ifdef PCST_GATED_IMPL
-template <class E, class O, bool NMN, bool MMN, int EPI, bool BIG>
+template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, bool BIG>
 int launch(GemmArgs& g, hipStream_t s) {
   constexpr int BM = BIG ? 256 : 128, BNH = BIG ? 128 : 64, WM = BIG ? 4 : 2, WN = 2;
   constexpr int NT = EPI == EPI_OUT ? 2 * BNH : BNH;
@@ -553,10 +582,21 @@ int launch(GemmArgs& g, hipStream_t s) {
   g.tiles_n = (int)tn;
   g.ntiles = (int)n;
   g.per_xcd = (int)cdiv(n, 8);
-  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, BM, BNH, WM, WN>), dim3((unsigned)(g.per_xcd * 8)),
+  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, ACT, BM, BNH, WM, WN>), dim3((unsigned)(g.per_xcd * 8)),
                      dim3(64 * WM * WN), 0, s, g);
   PCST_LAUNCH_CHECK("gated_linear");
   return PCST_OK;
+}
+
+// the forward and the recomputing backward, by activation and tile
+template <class E, class O, int EPI>
+int launch_gated(GemmArgs& g, hipStream_t s, int act) {
+  const bool big = take_big(g.M, g.N, 128);
+  if (act == ACT_SILU)
+    return big ? launch<E, O, false, false, EPI, ACT_SILU, true>(g, s) : launch<E, O, false, false, EPI, ACT_SILU, false>(g, s);
+  if (act == ACT_GELU)
+    return big ? launch<E, O, false, false, EPI, ACT_GELU, true>(g, s) : launch<E, O, false, false, EPI, ACT_GELU, false>(g, s);
+  return big ? launch<E, O, false, false, EPI, ACT_RELU, true>(g, s) : launch<E, O, false, false, EPI, ACT_RELU, false>(g, s);
 }
 
 inline GemmArgs fwd_args(const FwdCall& c) {
@@ -573,7 +613,6 @@ inline GemmArgs fwd_args(const FwdCall& c) {
   g.bg = c.bg;
   g.bu = c.bu;
   g.bias_f32 = c.bias_f32;
-  g.act = c.act;
   g.xs = c.xs;
   g.gs = c.gs;
   g.us = c.us;
@@ -585,8 +624,7 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
   GemmArgs g = fwd_args(c);
   g.out = c.h;
   g.ldo = c.F;
-  return take_big(c.M, c.F, 128) ? launch<E, O, false, false, EPI_FWD, true>(g, s)
-                                 : launch<E, O, false, false, EPI_FWD, false>(g, s);
+  return launch_gated<E, O, EPI_FWD>(g, s, c.act);
 }
 
 // dW's partials (a split's lie `stride` after the previous one's) added in order
@@ -631,8 +669,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   g.fpad = c.fpad;
   g.dh = c.dh;
   g.bpart = c.dbg || c.dbu ? c.bpart : nullptr;
-  int rc = take_big(f.M, f.F, 128) ? launch<E, T, false, false, EPI_BWD, true>(g, s)
-                                   : launch<E, T, false, false, EPI_BWD, false>(g, s);
+  int rc = launch_gated<E, T, EPI_BWD>(g, s, f.act);
   if (rc) return rc;
   if (g.bpart) {
     const dim3 grid((unsigned)cdiv(2 * f.F, 16));
@@ -660,8 +697,8 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.splits = d.groups = 1;
     d.out = c.dx;
     d.ldo = f.D;
-    rc = take_big(f.M, f.D, 256) ? launch<E, T, true, false, EPI_OUT, true>(d, s)
-                                 : launch<E, T, true, false, EPI_OUT, false>(d, s);
+    rc = take_big(f.M, f.D, 256) ? launch<E, T, true, false, EPI_OUT, 0, true>(d, s)
+                                 : launch<E, T, true, false, EPI_OUT, 0, false>(d, s);
     if (rc) return rc;
   }
   if (c.dwg || c.dwu) {
@@ -683,7 +720,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     w.out = c.wpart;
     w.o_group = f.F * f.D;
     w.o_split = 2 * f.F * f.D;
-    rc = p.big ? launch<E, float, true, true, EPI_OUT, true>(w, s) : launch<E, float, true, true, EPI_OUT, false>(w, s);
+    rc = p.big ? launch<E, float, true, true, EPI_OUT, 0, true>(w, s) : launch<E, float, true, true, EPI_OUT, 0, false>(w, s);
     if (rc) return rc;
     const int64_t n = f.F * f.D;
     const dim3 grid((unsigned)cdiv(n, 256));
