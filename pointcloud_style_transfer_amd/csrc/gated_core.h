@@ -55,9 +55,9 @@ struct GemmArgs {
   int tiles_m, tiles_n, ntiles, per_xcd;
   int splits;         // of k (row-contiguous operands only)
   int64_t kps;        // k per split
-  int groups;         // independent products of one launch (dWg, dWu): group g's A starts a_group bytes on
-  int64_t a_group, o_group, o_split;  // bytes, elements, elements
-  void* out;
+  int groups;         // independent products of one launch (dWg, dWu): group g's A starts a_group[g] bytes on
+  int64_t a_group[2], o_split;  // bytes; elements from one split's output to the next one's
+  void* out[2];       // per group
   int64_t ldo;        // elements
   const void *bg, *bu;
   int bias_f32;
@@ -247,22 +247,6 @@ struct Frag {
   }
 };
 
-// 4 consecutive outputs, the first n of them
-template <class O>
-__device__ __forceinline__ void store4(O* p, int n, f32x4 v) {
-  struct __attribute__((packed, aligned(sizeof(O)))) V4 { O v[4]; };
-  if (n >= 4) {
-    V4 q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = (O)v[i];
-    *reinterpret_cast<V4*>(p) = q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = (O)v[i];
-  }
-}
-
 template <class T>
 __device__ __forceinline__ void load_bias8(const void* b, int f32, int f, int n, float (&v)[8]) {
   if (!b || n <= 0) {
@@ -282,25 +266,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
   constexpr bool GATED = EPI != EPI_OUT;
   constexpr bool FAST = ES < 4;
+  constexpr bool LOOP = WM * WN == 4;  // several tiles a work-group
   static_assert(!GATED || !NMN, "the forward reads W with k contiguous");
   // one array per stage and operand, so that the compiler sees which loads a read has to wait for
   __shared__ __attribute__((aligned(1024))) char lds_a0[BM * kRowB], lds_a1[BM * kRowB];
   __shared__ __attribute__((aligned(1024))) char lds_b0[2 * BNH * kRowB], lds_b1[2 * BNH * kRowB];
-
-  // work-group L runs on XCD L % 8; an XCD's tiles follow each other in blocks of 4 row tiles, so that
-  // what its work-groups read at a time is shared in its L2
-  const int L = blockIdx.x;
-  int t = (L & 7) * g.per_xcd + (L >> 3);
-  if (t >= g.ntiles) return;
-  const int tiles_mn = g.tiles_m * g.tiles_n;
-  const int gs_ = t / tiles_mn;
-  t -= gs_ * tiles_mn;
-  const int group = gs_ % g.groups, split = gs_ / g.groups;
-  const int band = t / (4 * g.tiles_n), inb = t - band * 4 * g.tiles_n;
-  const int bh = g.tiles_m - 4 * band < 4 ? g.tiles_m - 4 * band : 4;
-  const int tm = 4 * band + inb % bh, tn = inb / bh;
-  const int64_t m0 = (int64_t)tm * BM;
-  const int n0 = tn * (GATED ? BNH : 2 * BNH);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -316,49 +286,73 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   fb[0].init(wn * 16 * TNH, lane);
   if (NMN) fb[NMN ? 1 : 0].init(BNH + wn * 16 * TNH, lane);
 
-  f32x4 acc[2][TNH][TM];
+  // LOOP: a work-group's tiles, one after the other; the next tile's first stage is loaded under the last
+  // products of this one and its epilogue, which needs no LDS (the large tiles have no registers left for
+  // it, and stages enough for the start of a tile not to matter).  Work-group L runs on XCD L % 8; an XCD's
+  // tiles follow each other in blocks of 4 row tiles, so that what its work-groups read at a time is
+  // shared in its L2.
+  struct Tile {
+    int64_t m0;
+    int n0, tm, group, split, nk, total;
+    int64_t klen;
+    const char *pa[2], *pb0[2], *pb1[2];  // per k segment, at its first k
+    int64_t ra, rb0, rb1;                 // bytes that may be read from there
+  };
+  auto decode = [&](int L, Tile& c) -> bool {
+    const int idx = L >> 3;
+    int t = (L & 7) * g.per_xcd + idx;
+    if (idx >= g.per_xcd || t >= g.ntiles) return false;
+    const int tiles_mn = g.tiles_m * g.tiles_n;
+    const int gs = t / tiles_mn;
+    t -= gs * tiles_mn;
+    c.group = g.groups > 1 ? gs % g.groups : 0;
+    c.split = g.groups > 1 ? gs / g.groups : gs;
+    const int band = t / (4 * g.tiles_n), inb = t - band * 4 * g.tiles_n;
+    const int bh = g.tiles_m - 4 * band < 4 ? g.tiles_m - 4 * band : 4;
+    const int tn = inb / bh;
+    c.tm = 4 * band + inb - tn * bh;
+    c.m0 = (int64_t)c.tm * BM;
+    c.n0 = tn * (GATED ? BNH : 2 * BNH);
+    const int64_t kb = c.split * g.kps;
+    c.klen = kb + g.kps < g.K ? g.kps : g.K - kb;
+    c.nk = (int)((c.klen + BKE - 1) / BKE);
+    c.total = c.nk * g.nseg;
+    const int64_t rows = g.M - c.m0 < BM ? g.M - c.m0 : BM;
+    const int64_t cols = g.N - c.n0 < BNH ? g.N - c.n0 : BNH;
+    const int64_t cols1 = GATED ? cols : g.N - c.n0 - BNH < BNH ? g.N - c.n0 - BNH : BNH;
+    c.ra = MMN ? c.klen * g.lda - c.m0 * ES : rows * g.lda - kb * ES;
+    c.rb0 = NMN ? c.klen * g.ldb - (int64_t)c.n0 * ES : cols * g.ldb - kb * ES;
+    c.rb1 = cols1 * g.ldb - kb * ES;  // (NMN: not used)
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int j = 0; j < TNH; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int64_t kb = (int64_t)split * g.kps;
-  const int64_t klen = kb + g.kps < g.K ? g.kps : g.K - kb;
-  const int nk = (int)((klen + BKE - 1) / BKE), total = nk * g.nseg;
-
-  auto load = [&](int it, PCST_LDS char* ia, PCST_LDS char* ib) {
-    const int seg = it >= nk && g.nseg > 1 ? 1 : 0;
-    const int64_t k = (int64_t)(it - seg * nk) * BKE;  // past klen: no bytes left
-    const char* a = g.a[seg] + group * g.a_group;
-    if (MMN)
-      sa.load(ia, a + (kb + k) * g.lda + m0 * ES, (klen - k) * g.lda - m0 * ES, 0, wave);
-    else
-      sa.load(ia, a + m0 * g.lda + (kb + k) * ES, k < klen ? (g.M - m0 < BM ? g.M - m0 : BM) * g.lda - (kb + k) * ES : 0,
-              (int)((klen - k) * ES < kRowB ? (klen - k) * ES : kRowB), wave);
-    if (NMN) {
-      sb.load(ib, g.b0[seg] + (kb + k) * g.ldb + (int64_t)n0 * ES, (klen - k) * g.ldb - (int64_t)n0 * ES, 0, wave);
-    } else {
-      const int kl = (int)((klen - k) * ES < kRowB ? (klen - k) * ES : kRowB);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int nh = GATED ? n0 : n0 + h * BNH;
-        const char* b = GATED && h ? g.b1[seg] : g.b0[seg];
-        const int rows = g.N - nh < BNH ? g.N - nh : BNH;
-        sb.load(ib + h * BNH * kRowB, b + (int64_t)nh * g.ldb + (kb + k) * ES,
-                rows <= 0 || k >= klen ? 0 : (int64_t)rows * g.ldb - (kb + k) * ES, kl, wave);
-      }
+    for (int q = 0; q < 2; ++q) {
+      c.pa[q] = g.a[q] + g.a_group[c.group] + (MMN ? kb * g.lda + c.m0 * ES : c.m0 * g.lda + kb * ES);
+      const int64_t ob = NMN ? kb * g.ldb + (int64_t)c.n0 * ES : (int64_t)c.n0 * g.ldb + kb * ES;
+      c.pb0[q] = g.b0[q] + ob;
+      c.pb1[q] = GATED ? g.b1[q] + ob : g.b0[q] + ob + (int64_t)BNH * g.ldb;
     }
+    return true;
+  };
+  const int64_t step_a = MMN ? BKE * g.lda : kRowB, step_b = NMN ? BKE * g.ldb : kRowB;
+  auto load = [&](const Tile& c, int it, PCST_LDS char* ia, PCST_LDS char* ib) {
+    const int seg = it >= c.nk && g.nseg > 1 ? 1 : 0;
+    const int k = it - (seg ? c.nk : 0);
+    const int64_t oa = k * step_a, ob = k * step_b;
+    const int64_t left = c.klen * ES - (int64_t)k * kRowB;
+    const int kl = left > kRowB ? kRowB : (int)left;
+    sa.load(ia, c.pa[seg] + oa, c.ra - oa, kl, wave);
+    sb.load(ib, c.pb0[seg] + ob, c.rb0 - ob, kl, wave);
+    if (!NMN) sb.load(ib + BNH * kRowB, c.pb1[seg] + ob, c.rb1 - ob, kl, wave);
   };
 
-  auto compute = [&](const PCST_LDS char* ia, const PCST_LDS char* ib) {
+  f32x4 acc[2][TNH][TM];
+  auto compute = [&](const PCST_LDS char* ia, const PCST_LDS char* ib, auto&& prefetch) {
     if constexpr (ES == 1) {
       i32x4 a[2][TM];
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int i = 0; i < TM; ++i) a[ks][i] = fa.read(ia, i, ks);
+      prefetch();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -390,6 +384,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
       read_b(0, 0);
       read_b(0, 1);
       __builtin_amdgcn_sched_barrier(0);
+      prefetch();  // the other stage's loads, behind this one's first reads
       mma(0, 0);
       read_a(1);
       __builtin_amdgcn_sched_barrier(0);
@@ -407,23 +402,46 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   PCST_LDS char* a1 = (PCST_LDS char*)lds_a1;
   PCST_LDS char* b0 = (PCST_LDS char*)lds_b0;
   PCST_LDS char* b1 = (PCST_LDS char*)lds_b1;
-  // pairs of stages in one basic block (the accumulators stay in place); a load past the last stage
-  // fetches nothing
   auto next = [&]() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the stage
     __syncthreads();                                  // everyone's; and the other stage has been read
   };
-  load(0, a0, b0);
-  for (int it = 0; it + 2 <= total; it += 2) {
+  Tile cur, nxt;
+  int L = blockIdx.x;
+  if (!decode(L, cur)) return;
+  load(cur, 0, a0, b0);
+  bool more = LOOP;
+  do {
+    if (LOOP) {
+      L += gridDim.x;
+      more = decode(L, nxt);
+      if (!more) nxt = cur;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < TNH; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // pairs of stages in one basic block: the accumulators stay in place
+    for (int it = 0; it + (LOOP ? 3 : 2) <= cur.total; it += 2) {
+      next();
+      compute(a0, b0, [&]() { load(cur, it + 1, a1, b1); });
+      next();
+      compute(a1, b1, [&]() { load(cur, it + 2, a0, b0); });  // past the last stage: fetches nothing
+    }
+    const int64_t m0 = cur.m0;
+    const int n0 = cur.n0, tm = cur.tm;
     next();
-    load(it + 1, a1, b1);
-    compute(a0, b0);
-    next();
-    load(it + 2, a0, b0);
-    compute(a1, b1);
-  }
-  next();
-  if (total & 1) compute(a0, b0);
+    if (cur.total & 1) {
+      compute(a0, b0, []() {});
+      if (LOOP) __syncthreads();
+      if (LOOP && more) load(nxt, 0, a0, b0);
+    } else if (LOOP) {
+      compute(a0, b0, [&]() { load(cur, cur.total - 1, a1, b1); });
+      next();
+      compute(a1, b1, [&]() { if (more) load(nxt, 0, a0, b0); });
+    }
 
   // ---- epilogue
   const int l = lane & 15, q = lane >> 4;
@@ -470,7 +488,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
             float o[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) o[k] = act_value<FAST, ACT>(gv[k]) * uv[k];
-            store8(static_cast<O*>(g.out) + m * g.ldo + f, n, o);
+            store8(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
           }
         } else if (m < g.M && f < g.fpad) {
           float d[8], og[8], ou[8];
@@ -489,7 +507,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
             csum[0][k] += og[k];
             csum[1][k] += ou[k];
           }
-          O* o = static_cast<O*>(g.out) + m * g.ldo + f;
+          O* o = static_cast<O*>(g.out[0]) + m * g.ldo + f;
           store8(o, 8, og);
           store8(o + g.fpad, 8, ou);
         }
@@ -508,7 +526,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
       }
     }
   } else {
-    O* out = static_cast<O*>(g.out) + group * g.o_group + split * g.o_split;
+    O* out = static_cast<O*>(g.out[cur.group]) + cur.split * g.o_split;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int64_t m = m0 + wm * 16 * TM + 16 * i + l;
@@ -518,10 +536,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int j = 0; j < TNH; ++j) {
           const int n = n0 + h * BNH + wn * 16 * TNH + (NMN ? 16 * j + 4 * q : q * 4 * TNH + 4 * j);
-          if (n < g.N) store4(out + m * g.ldo + n, g.N - n, acc[h][j][i]);
+          if (n >= g.N) continue;
+          const float v[4] = {acc[h][j][i][0], acc[h][j][i][1], acc[h][j][i][2], acc[h][j][i][3]};
+          store_n<O, 4>(out + m * g.ldo + n, g.N - n, v);
         }
     }
   }
+    cur = nxt;
+  } while (LOOP && more);
 }
 
 // ---- host side of one operand type
@@ -545,7 +567,7 @@ struct BwdCall {
 
 constexpr int kBigTiles = 200;  // launches of at least this many large tiles take them
 
-inline bool take_big(int64_t M, int64_t N, int nw) { return cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
+inline bool take_big(int64_t M, int64_t N, int nw, int64_t kbytes) { return kbytes >= 1024 && cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
 
 struct WgradPlan {
   bool big;
@@ -564,7 +586,7 @@ inline WgradPlan wgrad_plan(int64_t M, int64_t D, int64_t F, int es) {
   p.splits = (int)std::max<int64_t>(1, cdiv(M, p.kps));
   return p;
 }
-inline int64_t bias_parts(int64_t M, int64_t F) { return take_big(M, F, 128) ? cdiv(M, 256) * 4 : cdiv(M, 128) * 2; }
+inline int64_t bias_parts(int64_t M, int64_t F, int64_t kbytes) { return take_big(M, F, 128, kbytes) ? cdiv(M, 256) * 4 : cdiv(M, 128) * 2; }
 
 template <class E>
 int fwd(const FwdCall& c, void* stream);
@@ -582,7 +604,9 @@ int launch(GemmArgs& g, hipStream_t s) {
   g.tiles_n = (int)tn;
   g.ntiles = (int)n;
   g.per_xcd = (int)cdiv(n, 8);
-  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, ACT, BM, BNH, WM, WN>), dim3((unsigned)(g.per_xcd * 8)),
+  // small tiles: as many work-groups as run at a time (two on each of 256 CUs)
+  const unsigned grid = (unsigned)(BIG ? g.per_xcd * 8 : std::min<int64_t>(g.per_xcd * 8, 512));
+  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, ACT, BM, BNH, WM, WN>), dim3(grid),
                      dim3(64 * WM * WN), 0, s, g);
   PCST_LAUNCH_CHECK("gated_linear");
   return PCST_OK;
@@ -591,7 +615,7 @@ int launch(GemmArgs& g, hipStream_t s) {
 // the forward and the recomputing backward, by activation and tile
 template <class E, class O, int EPI>
 int launch_gated(GemmArgs& g, hipStream_t s, int act) {
-  const bool big = take_big(g.M, g.N, 128);
+  const bool big = take_big(g.M, g.N, 128, g.K * elem_size<E>());
   if (act == ACT_SILU)
     return big ? launch<E, O, false, false, EPI, ACT_SILU, true>(g, s) : launch<E, O, false, false, EPI, ACT_SILU, false>(g, s);
   if (act == ACT_GELU)
@@ -622,21 +646,22 @@ inline GemmArgs fwd_args(const FwdCall& c) {
 template <class E, class O>
 int fwd_out(const FwdCall& c, hipStream_t s) {
   GemmArgs g = fwd_args(c);
-  g.out = c.h;
+  g.out[0] = c.h;
   g.ldo = c.F;
   return launch_gated<E, O, EPI_FWD>(g, s, c.act);
 }
 
-// dW's partials (a split's lie `stride` after the previous one's) added in order
+// dW's partials (one of n values per split and matrix) added in order; blockIdx.y: the matrix
 template <class O>
-__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, int64_t n, int64_t stride,
-                                                      int parts, O* __restrict__ out) {
+__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, int64_t n, int parts,
+                                                      O* __restrict__ out0, O* __restrict__ out1) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= n) return;
+  part += blockIdx.y * n + e;
   float s = 0.0f;
 #pragma unroll 8
-  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * stride + e];
-  out[e] = (O)s;
+  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * gridDim.y * n];
+  (blockIdx.y ? out1 : out0)[e] = (O)s;
 }
 // 16 columns a work-group, 16 slices of the parts
 template <class O>
@@ -658,13 +683,18 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ par
   }
 }
 
+template <class E, class O>
+int wgrad_launch(GemmArgs& w, bool big, hipStream_t s) {
+  return big ? launch<E, O, true, true, EPI_OUT, 0, true>(w, s) : launch<E, O, true, true, EPI_OUT, 0, false>(w, s);
+}
+
 template <class E>
 int bwd_impl(const BwdCall& c, hipStream_t s) {
   typedef typename E::T T;
   constexpr int ES = elem_size<E>();
   const FwdCall& f = c.f;
   GemmArgs g = fwd_args(f);
-  g.out = c.dgu;
+  g.out[0] = c.dgu;
   g.ldo = 2 * c.fpad;
   g.fpad = c.fpad;
   g.dh = c.dh;
@@ -673,7 +703,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   if (rc) return rc;
   if (g.bpart) {
     const dim3 grid((unsigned)cdiv(2 * f.F, 16));
-    const int parts = (int)bias_parts(f.M, f.F);
+    const int parts = (int)bias_parts(f.M, f.F, f.D * ES);
     if (c.bgrad_f32)
       hipLaunchKernelGGL(bias_kernel<float>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts,
                          static_cast<float*>(c.dbg), static_cast<float*>(c.dbu));
@@ -695,9 +725,9 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.K = d.kps = f.F;
     d.nseg = 2;
     d.splits = d.groups = 1;
-    d.out = c.dx;
+    d.out[0] = c.dx;
     d.ldo = f.D;
-    rc = take_big(f.M, f.D, 256) ? launch<E, T, true, false, EPI_OUT, 0, true>(d, s)
+    rc = take_big(f.M, f.D, 256, 2 * f.F * ES) ? launch<E, T, true, false, EPI_OUT, 0, true>(d, s)
                                  : launch<E, T, true, false, EPI_OUT, 0, false>(d, s);
     if (rc) return rc;
   }
@@ -714,27 +744,33 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     w.kps = p.kps;
     w.nseg = 1;
     w.splits = p.splits;
-    w.groups = 2;
-    w.a_group = c.fpad * ES;
     w.ldo = f.D;
-    w.out = c.wpart;
-    w.o_group = f.F * f.D;
-    w.o_split = 2 * f.F * f.D;
-    rc = p.big ? launch<E, float, true, true, EPI_OUT, 0, true>(w, s) : launch<E, float, true, true, EPI_OUT, 0, false>(w, s);
-    if (rc) return rc;
-    const int64_t n = f.F * f.D;
-    const dim3 grid((unsigned)cdiv(n, 256));
-    for (int k = 0; k < 2; ++k) {
-      void* o = k ? c.dwu : c.dwg;
-      if (!o) continue;
+    void* outs[2] = {c.dwg, c.dwu};
+    for (int k = 0; k < 2; ++k)
+      if (outs[k]) {
+        w.a_group[w.groups] = k * c.fpad * ES;
+        w.out[w.groups++] = outs[k];
+      }
+    if (p.splits == 1) {
+      rc = c.wgrad_f32 ? wgrad_launch<E, float>(w, p.big, s) : wgrad_launch<E, T>(w, p.big, s);
+      if (rc) return rc;
+    } else {
+      const int64_t n = f.F * f.D;
+      void *o0 = w.out[0], *o1 = w.out[1];
+      w.out[0] = c.wpart;
+      w.out[1] = c.wpart + n;
+      w.o_split = w.groups * n;
+      rc = wgrad_launch<E, float>(w, p.big, s);
+      if (rc) return rc;
+      const dim3 grid((unsigned)cdiv(n, 256), (unsigned)w.groups);
       if (c.wgrad_f32)
-        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, s, c.wpart + k * n, n, 2 * n, p.splits,
-                           static_cast<float*>(o));
+        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, s, c.wpart, n, p.splits,
+                           static_cast<float*>(o0), static_cast<float*>(o1));
       else
-        hipLaunchKernelGGL(combine_kernel<T>, grid, dim3(256), 0, s, c.wpart + k * n, n, 2 * n, p.splits,
-                           static_cast<T*>(o));
+        hipLaunchKernelGGL(combine_kernel<T>, grid, dim3(256), 0, s, c.wpart, n, p.splits, static_cast<T*>(o0),
+                           static_cast<T*>(o1));
+      PCST_LAUNCH_CHECK("gated_linear_bwd");
     }
-    PCST_LAUNCH_CHECK("gated_linear_bwd");
   }
   return PCST_OK;
 }

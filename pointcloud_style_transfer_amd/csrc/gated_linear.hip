@@ -51,7 +51,7 @@ Layout lay(void* ws, int dt, int64_t M, int64_t D, int64_t F, bool bwd) {
   l.fpad = cdiv(F, 64) * 64;
   if (bwd) {
     l.dgu = c.take<char>((size_t)(M * 2 * l.fpad * es));
-    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, F) * 2 * F));
+    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, F, D * es) * 2 * F));
     l.wpart = c.take<float>((size_t)(gated::wgrad_plan(M, D, F, es).splits * 2 * F * D));
   }
   l.bytes = c.bytes();

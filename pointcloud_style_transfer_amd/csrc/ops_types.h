@@ -26,37 +26,48 @@ __device__ __forceinline__ float to_f32(T v) {
   return (float)v;
 }
 
-// 8 consecutive elements at any element-aligned address: one or two 16-byte accesses (the hardware
-// takes global accesses of any alignment), the first n elementwise where the row ends inside
-template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) Vec8 {
-  T v[8];
+// 8 (4) consecutive elements at any element-aligned address as vector accesses (the hardware takes
+// global accesses of any alignment), the first n elementwise where the row ends inside.  Vector types,
+// not arrays: an array's eight elements are split up again and leave as narrow accesses.
+template <class T, int N>
+struct Vec {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef V Any __attribute__((aligned(sizeof(T))));
 };
 
-template <class T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-  if (n >= 8) {
-    const Vec8<T> q = *reinterpret_cast<const Vec8<T>*>(p);
+template <class T, int N>
+__device__ __forceinline__ void load_n(const T* p, int n, float (&v)[N]) {
+  if (n >= N) {
+    const typename Vec<T, N>::V q = *reinterpret_cast<const typename Vec<T, N>::Any*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)q.v[i];
+    for (int i = 0; i < N; ++i) v[i] = (float)q[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+    for (int i = 0; i < N; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+  }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_n(T* p, int n, const float (&v)[N]) {
+  if (n >= N) {
+    typename Vec<T, N>::V q;
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = (T)v[i];
+    *reinterpret_cast<typename Vec<T, N>::Any*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (T)v[i];
   }
 }
 
 template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+  load_n<T, 8>(p, n, v);
+}
+template <class T>
 __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-  if (n >= 8) {
-    Vec8<T> q;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q.v[i] = (T)v[i];
-    *reinterpret_cast<Vec8<T>*>(p) = q;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (T)v[i];
-  }
+  store_n<T, 8>(p, n, v);
 }
 
 // 8 floats -> 8 e4m3 values (round to nearest even); NaN stays NaN
