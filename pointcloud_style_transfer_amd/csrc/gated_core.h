@@ -51,7 +51,6 @@ struct GemmArgs {
   int64_t M;          // rows (per group)
   int N;              // columns of a column block's matrix
   int64_t K;          // per segment
-  int nseg;
   int tiles_m, tiles_n, ntiles, per_xcd;
   int splits;         // of k (row-contiguous operands only)
   int64_t kps;        // k per split
@@ -266,6 +265,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
   constexpr bool GATED = EPI != EPI_OUT;
   constexpr bool FAST = ES < 4;
+  constexpr int NSEG = NMN && !MMN ? 2 : 1;  // k segments: dx sums over Wg, then over Wu
   constexpr bool LOOP = WM * WN == 4;  // several tiles a work-group
   static_assert(!GATED || !NMN, "the forward reads W with k contiguous");
   // one array per stage and operand, so that the compiler sees which loads a read has to wait for
@@ -294,8 +294,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   struct Tile {
     int64_t m0;
     int n0, tm, group, split, nk, total;
-    int64_t klen;
-    const char *pa[2], *pb0[2], *pb1[2];  // per k segment, at its first k
+    int64_t klen;  // of a segment
+    const char *pa[NSEG], *pb0[NSEG], *pb1[NSEG];  // per k segment, at its first k
     int64_t ra, rb0, rb1;                 // bytes that may be read from there
   };
   auto decode = [&](int L, Tile& c) -> bool {
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     const int64_t kb = c.split * g.kps;
     c.klen = kb + g.kps < g.K ? g.kps : g.K - kb;
     c.nk = (int)((c.klen + BKE - 1) / BKE);
-    c.total = c.nk * g.nseg;
+    c.total = c.nk * NSEG;
     const int64_t rows = g.M - c.m0 < BM ? g.M - c.m0 : BM;
     const int64_t cols = g.N - c.n0 < BNH ? g.N - c.n0 : BNH;
     const int64_t cols1 = GATED ? cols : g.N - c.n0 - BNH < BNH ? g.N - c.n0 - BNH : BNH;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
     c.rb0 = NMN ? c.klen * g.ldb - (int64_t)c.n0 * ES : cols * g.ldb - kb * ES;
     c.rb1 = cols1 * g.ldb - kb * ES;  // (NMN: not used)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < NSEG; ++q) {
       c.pa[q] = g.a[q] + g.a_group[c.group] + (MMN ? kb * g.lda + c.m0 * ES : c.m0 * g.lda + kb * ES);
       const int64_t ob = NMN ? kb * g.ldb + (int64_t)c.n0 * ES : (int64_t)c.n0 * g.ldb + kb * ES;
       c.pb0[q] = g.b0[q] + ob;
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   };
   const int64_t step_a = MMN ? BKE * g.lda : kRowB, step_b = NMN ? BKE * g.ldb : kRowB;
   auto load = [&](const Tile& c, int it, PCST_LDS char* ia, PCST_LDS char* ib) {
-    const int seg = it >= c.nk && g.nseg > 1 ? 1 : 0;
+    const int seg = NSEG > 1 && it >= c.nk ? 1 : 0;
     const int k = it - (seg ? c.nk : 0);
     const int64_t oa = k * step_a, ob = k * step_b;
     const int64_t left = c.klen * ES - (int64_t)k * kRowB;
@@ -404,19 +404,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   PCST_LDS char* b1 = (PCST_LDS char*)lds_b1;
   auto next = [&]() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the stage
-    __syncthreads();                                  // everyone's; and the other stage has been read
+    __builtin_amdgcn_s_barrier();                     // everyone's; and the other stage has been read
+    asm volatile("" ::: "memory");
+  };
+  // The same at the start of a tile, whose stage was loaded before the previous tile's stores: these stay
+  // in flight.  kStores of them follow the loads where that tile was a whole one (`stores`); the counter
+  // falls in order, so at kStores left, the loads are done.
+  constexpr int kStores = EPI == EPI_FWD ? TM * TNH / 2 : TM * TNH * 2;
+  auto first = [&](bool stores) {
+    if (stores && LOOP && EPI != EPI_BWD)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
   Tile cur, nxt;
   int L = blockIdx.x;
   if (!decode(L, cur)) return;
   load(cur, 0, a0, b0);
-  bool more = LOOP;
+  bool more = LOOP, stores = false;
   do {
-    if (LOOP) {
-      L += gridDim.x;
-      more = decode(L, nxt);
-      if (!more) nxt = cur;
-    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -424,24 +432,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     // pairs of stages in one basic block: the accumulators stay in place
+    first(stores);
     for (int it = 0; it + (LOOP ? 3 : 2) <= cur.total; it += 2) {
-      next();
       compute(a0, b0, [&]() { load(cur, it + 1, a1, b1); });
       next();
       compute(a1, b1, [&]() { load(cur, it + 2, a0, b0); });  // past the last stage: fetches nothing
+      next();
     }
     const int64_t m0 = cur.m0;
     const int n0 = cur.n0, tm = cur.tm;
-    next();
+    if (LOOP) {
+      L += gridDim.x;
+      more = decode(L, nxt);
+    }
     if (cur.total & 1) {
       compute(a0, b0, []() {});
-      if (LOOP) __syncthreads();
+      if (LOOP) next();
       if (LOOP && more) load(nxt, 0, a0, b0);
     } else if (LOOP) {
       compute(a0, b0, [&]() { load(cur, cur.total - 1, a1, b1); });
       next();
       compute(a1, b1, [&]() { if (more) load(nxt, 0, a0, b0); });
     }
+
+    asm volatile("" ::: "memory");  // the next tile's loads stay ahead of the stores
+    stores = m0 + BM <= g.M && n0 + (GATED ? BNH : 2 * BNH) <= g.N;
 
   // ---- epilogue
   const int l = lane & 15, q = lane >> 4;
@@ -542,7 +557,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
         }
     }
   }
-    cur = nxt;
+    if (LOOP) cur = nxt;
   } while (LOOP && more);
 }
 
@@ -633,7 +648,7 @@ inline GemmArgs fwd_args(const FwdCall& c) {
   g.M = c.M;
   g.N = (int)c.F;
   g.K = g.kps = c.D;
-  g.nseg = g.splits = g.groups = 1;
+  g.splits = g.groups = 1;
   g.bg = c.bg;
   g.bu = c.bu;
   g.bias_f32 = c.bias_f32;
@@ -723,7 +738,6 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.M = f.M;
     d.N = (int)f.D;
     d.K = d.kps = f.F;
-    d.nseg = 2;
     d.splits = d.groups = 1;
     d.out[0] = c.dx;
     d.ldo = f.D;
@@ -742,7 +756,6 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     w.N = (int)f.D;
     w.K = f.M;
     w.kps = p.kps;
-    w.nseg = 1;
     w.splits = p.splits;
     w.ldo = f.D;
     void* outs[2] = {c.dwg, c.dwu};
