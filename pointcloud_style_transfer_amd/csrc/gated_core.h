@@ -19,9 +19,10 @@
 // operands whose rows are contiguous -- spread over the banks.  Loads past a tile's rows or past k are
 // sent past the buffer's end and arrive as zeros, so ragged sizes take no other path.
 //
-// The MFMA takes B's rows as its row operand, so a lane's four accumulators are four consecutive output
-// columns; with k contiguous, the rows of a wave's tiles are dealt so that a lane's tiles follow each
-// other as well: 4 * TNH consecutive outputs a lane, whole lines a wave, and no pass through LDS.
+// Outputs go to memory from the accumulators, 16 lanes side by side in a row: what counts is how many
+// pieces a store falls into (16 rows a store: 1.9 M requests of 32 bytes for 60000 x 512 bf16, and twice
+// the time).  In the forward, W's rows are dealt to the tiles so that a lane's tiles are consecutive
+// features and 16 lanes a whole 128-byte line.
 #pragma once
 #include "ops_types.h"
 
@@ -145,15 +146,9 @@ __device__ __forceinline__ float act_grad(float g, float& value) {
   return g > 0.0f ? 1.0f : g * 0.0f;
 }
 
-// ---- LDS images.  KC: row r holds 128 bytes of k; piece c of 16 bytes at position c ^ swz(r).
-// Row operand: 16 lanes read rows 16 i + 0..15 -> swz = (r >> 1) & 7.
-// Column operand: 16 lanes read rows (l >> 2) * 4 TNH + (l & 3) -> bits 1 and log2(4 TNH), + 1.
-template <int TNH, bool COL>
-__device__ __forceinline__ int swz_kc(int r) {
-  if (!COL) return (r >> 1) & 7;
-  constexpr int S = TNH == 4 ? 4 : 3;
-  return ((r >> 1) & 1) | (((r >> S) & 3) << 1);
-}
+// ---- LDS images.  KC: row r holds 128 bytes of k; piece c of 16 bytes at position c ^ swz(r), so that the
+// 16 lanes that read the same piece of 16 consecutive rows meet every bank once
+__device__ __forceinline__ int swz_kc(int r) { return (r >> 1) & 7; }
 // MN: row k holds W elements; 16-bit: transposed reads of rows k..k+3 (a group of 16 lanes) at 32
 // bytes; fp32: 16 lanes read 64 bytes of one row, the four groups rows 4 apart
 template <int ES, int CPR>
@@ -162,8 +157,10 @@ __device__ __forceinline__ int swz_mn(int k) {
   return (4 * ((k >> 2) & 3)) & (CPR - 1);
 }
 
-// One operand's image of R rows (KC) or R columns (MN): R * 128 bytes either way
-template <class E, bool MN, bool COL, int R, int TNH, int NW>
+// One operand's image of R rows (KC) or R columns (MN): R * 128 bytes either way.  DEAL > 1 (KC): row
+// 16 t + j of each 16 * DEAL rows of the image is row DEAL j + t of the operand, so that lane j of a wave's
+// DEAL tiles holds DEAL consecutive outputs.
+template <class E, bool MN, int R, int DEAL, int NW>
 struct Stage {
   static constexpr int ES = elem_size<E>();
   static constexpr int RB = R * ES;          // MN: bytes of one k row
@@ -183,8 +180,9 @@ struct Stage {
         piece[j] = 0;
       } else {
         const int r = at / kRowB, p = (at % kRowB) / 16;
-        piece[j] = (p ^ swz_kc<TNH, COL>(r)) * 16;
-        off[j] = (uint32_t)(r * ld + piece[j]);
+        piece[j] = (p ^ swz_kc(r)) * 16;
+        const int w = r % (16 * DEAL);
+        off[j] = (uint32_t)((r - w + w % 16 * DEAL + w / 16) * ld + piece[j]);
       }
     }
   }
@@ -200,9 +198,8 @@ struct Stage {
   }
 };
 
-// Fragment reads of one wave: T tiles of 16 rows from row r0 on (COL: dealt as 4 T consecutive rows a
-// lane group); a lane gets 16 bytes of k of step ks
-template <class E, bool MN, bool COL, int R, int T, int TNH>
+// Fragment reads of one wave: T tiles of 16 rows from row r0 on; a lane gets 16 bytes of k of step ks
+template <class E, bool MN, int R, int T>
 struct Frag {
   static constexpr int ES = elem_size<E>();
   static constexpr int RB = R * ES, CPR = RB / 16;
@@ -223,9 +220,9 @@ struct Frag {
         }
       }
     } else {
-      const int r = r0 + (COL ? (l >> 2) * 4 * TNH + (l & 3) : l);
+      const int r = r0 + l;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) at[ks] = r * kRowB + (((ks * 4 + g) ^ swz_kc<TNH, COL>(r)) * 16);
+      for (int ks = 0; ks < 2; ++ks) at[ks] = r * kRowB + (((ks * 4 + g) ^ swz_kc(r)) * 16);
     }
   }
   __device__ __forceinline__ i32x4 read(const PCST_LDS char* img, int t, int ks) const {
@@ -242,19 +239,20 @@ struct Frag {
       }
       return v;
     }
-    return *(const PCST_LDS i32x4*)(img + at[MN ? 0 : ks] + t * (COL ? 4 : 16) * kRowB);
+    return *(const PCST_LDS i32x4*)(img + at[MN ? 0 : ks] + t * 16 * kRowB);
   }
 };
 
-template <class T>
-__device__ __forceinline__ void load_bias8(const void* b, int f32, int f, int n, float (&v)[8]) {
+// N values of a vector of T or float from f on, n of them there; zeros elsewhere and for no vector
+template <class T, int N>
+__device__ __forceinline__ void load_bias(const void* b, int f32, int64_t f, int n, float (&v)[N]) {
   if (!b || n <= 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int i = 0; i < N; ++i) v[i] = 0.0f;
   } else if (f32) {
-    load8(static_cast<const float*>(b) + f, n, v);
+    load_n<float, N>(static_cast<const float*>(b) + f, n, v);
   } else {
-    load8(static_cast<const T*>(b) + f, n, v);
+    load_n<T, N>(static_cast<const T*>(b) + f, n, v);
   }
 }
 
@@ -276,12 +274,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  Stage<E, MMN, false, BM, TNH, NW> sa;
-  Stage<E, NMN, true, NMN ? 2 * BNH : BNH, TNH, NW> sb;
+  Stage<E, MMN, BM, 1, NW> sa;
+  Stage<E, NMN, NMN ? 2 * BNH : BNH, NMN ? 1 : TNH, NW> sb;
   sa.init(wave, lane, g.lda);
   sb.init(wave, lane, g.ldb);
-  Frag<E, MMN, false, BM, TM, TNH> fa;
-  Frag<E, NMN, true, NMN ? 2 * BNH : BNH, TNH, TNH> fb[NMN ? 2 : 1];
+  Frag<E, MMN, BM, TM> fa;
+  Frag<E, NMN, NMN ? 2 * BNH : BNH, TNH> fb[NMN ? 2 : 1];
   fa.init(wm * 16 * TM, lane);
   fb[0].init(wn * 16 * TNH, lane);
   if (NMN) fb[NMN ? 1 : 0].init(BNH + wn * 16 * TNH, lane);
@@ -359,7 +357,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
         for (int j = 0; j < TNH; ++j) {
           const i32x4 b0 = fb[0].read(ib + h * BNH * kRowB, j, 0), b1 = fb[0].read(ib + h * BNH * kRowB, j, 1);
 #pragma unroll
-          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma32_e4m3(b0, b1, a[0][i], a[1][i], acc[h][j][i]);
+          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma32_e4m3(a[0][i], a[1][i], b0, b1, acc[h][j][i]);
         }
     } else {
       // four groups (k step, column block) of TM * TNH products; a group's products run while the next
@@ -378,7 +376,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int j = 0; j < TNH; ++j)
 #pragma unroll
-          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma16<E>(b[h][j], a[ks][i], acc[h][j][i]);
+          for (int i = 0; i < TM; ++i) acc[h][j][i] = GATED ? mma16<E>(a[ks][i], b[h][j], acc[h][j][i]) : mma16<E>(b[h][j], a[ks][i], acc[h][j][i]);
       };
       read_a(0);
       read_b(0, 0);
@@ -410,7 +408,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   // The same at the start of a tile, whose stage was loaded before the previous tile's stores: these stay
   // in flight.  kStores of them follow the loads where that tile was a whole one (`stores`); the counter
   // falls in order, so at kStores left, the loads are done.
-  constexpr int kStores = EPI == EPI_FWD ? TM * TNH / 2 : TM * TNH * 2;
+  constexpr int kStores = EPI == EPI_FWD ? TM * 4 : TM * TNH * 2;
   auto first = [&](bool stores) {
     if (stores && LOOP && EPI != EPI_BWD)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
@@ -461,83 +459,72 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   // ---- epilogue
   const int l = lane & 15, q = lane >> 4;
   if constexpr (GATED) {
-    constexpr int RUN = 4 * TNH;  // consecutive features of a lane
-    const int f0 = n0 + wn * 16 * TNH + q * RUN;
-    const int nf = g.N - f0;
+    // lane: row 4 q + r of each row tile, TNH consecutive features
+    const int f = n0 + (wn * 16 + l) * TNH, n = g.N - f;
+    float bg[TNH], bu[TNH], sg[TNH], su[TNH], cg[TNH], cu[TNH];
+    load_bias<O, TNH>(g.bg, g.bias_f32, f, n, bg);
+    load_bias<O, TNH>(g.bu, g.bias_f32, f, n, bu);
+    if (ES == 1) {
+      load_bias<float, TNH>(g.gs, 1, f, n, sg);
+      load_bias<float, TNH>(g.us, 1, f, n, su);
+    }
 #pragma unroll
-    for (int p = 0; p < RUN / 8; ++p) {
-      const int f = f0 + 8 * p, n = nf - 8 * p;
-      float bg[8], bu[8], sg[8], su[8], csum[2][8];
+    for (int t = 0; t < TNH; ++t) cg[t] = cu[t] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) csum[0][k] = csum[1][k] = 0.0f;
-      load_bias8<O>(g.bg, g.bias_f32, f, n, bg);
-      load_bias8<O>(g.bu, g.bias_f32, f, n, bu);
-      if (ES == 1) {
-        load_bias8<float>(g.gs, 1, f, n, sg);
-        load_bias8<float>(g.us, 1, f, n, su);
-      }
+    for (int i = 0; i < TM; ++i) {
+      const int64_t mi = m0 + wm * 16 * TM + 16 * i + 4 * q;
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int64_t m = m0 + wm * 16 * TM + 16 * i + l;
-        float gv[8], uv[8];
+      for (int r = 0; r < 4; ++r) {
+        const int64_t m = mi + r;
+        if (m >= g.M) continue;
+        float gv[TNH], uv[TNH];
+        const float xs = ES == 1 ? g.xs[m] : 1.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          gv[k] = acc[0][2 * p + k / 4][i][k % 4];
-          uv[k] = acc[1][2 * p + k / 4][i][k % 4];
-        }
-        if (ES == 1) {
-          const float xs = m < g.M ? g.xs[m] : 0.0f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            gv[k] *= xs * sg[k];
-            uv[k] *= xs * su[k];
+        for (int t = 0; t < TNH; ++t) {
+          gv[t] = acc[0][t][i][r];
+          uv[t] = acc[1][t][i][r];
+          if (ES == 1) {
+            gv[t] *= xs * sg[t];
+            uv[t] *= xs * su[t];
           }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          gv[k] += bg[k];
-          uv[k] += bu[k];
+          gv[t] += bg[t];
+          uv[t] += bu[t];
         }
         if (EPI == EPI_FWD) {
-          if (m < g.M && n > 0) {
-            float o[8];
+          float o[TNH];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = act_value<FAST, ACT>(gv[k]) * uv[k];
-            store8(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
-          }
-        } else if (m < g.M && f < g.fpad) {
-          float d[8], og[8], ou[8];
-          if (n > 0) {
-            load8(static_cast<const O*>(g.dh) + m * g.N + f, n, d);
-          } else {
+          for (int t = 0; t < TNH; ++t) o[t] = act_value<FAST, ACT>(gv[t]) * uv[t];
+          if (n > 0) store_n<O, TNH>(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
+        } else if (f < g.fpad) {
+          float d[TNH], og[TNH], ou[TNH];
+          load_bias<O, TNH>(g.dh, 0, m * g.N + f, n, d);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) d[k] = 0.0f;
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int t = 0; t < TNH; ++t) {
             float v;
-            const float da = act_grad<FAST, ACT>(gv[k], v);
-            og[k] = k < n ? d[k] * uv[k] * da : 0.0f;  // the padding up to fpad is zero
-            ou[k] = k < n ? d[k] * v : 0.0f;
-            csum[0][k] += og[k];
-            csum[1][k] += ou[k];
+            const float da = act_grad<FAST, ACT>(gv[t], v);
+            og[t] = t < n ? d[t] * uv[t] * da : 0.0f;  // the padding up to fpad is zero
+            ou[t] = t < n ? d[t] * v : 0.0f;
+            cg[t] += og[t];
+            cu[t] += ou[t];
           }
           O* o = static_cast<O*>(g.out[0]) + m * g.ldo + f;
-          store8(o, 8, og);
-          store8(o + g.fpad, 8, ou);
+          store_n<O, TNH>(o, TNH, og);
+          store_n<O, TNH>(o + g.fpad, TNH, ou);
         }
       }
-      if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
-        float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N + f;
+    }
+    if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
+      float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N + f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float v = csum[h][k];
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-            if (l == 0 && k < n) bp[(int64_t)h * g.N + k] = v;
-          }
+      for (int t = 0; t < TNH; ++t) {
+        cg[t] += __shfl_xor(cg[t], 16, 64);
+        cg[t] += __shfl_xor(cg[t], 32, 64);
+        cu[t] += __shfl_xor(cu[t], 16, 64);
+        cu[t] += __shfl_xor(cu[t], 32, 64);
+        if (q == 0 && t < n) {
+          bp[t] = cg[t];
+          bp[g.N + t] = cu[t];
+        }
       }
     }
   } else {
@@ -582,7 +569,7 @@ struct BwdCall {
 
 constexpr int kBigTiles = 200;  // launches of at least this many large tiles take them
 
-inline bool take_big(int64_t M, int64_t N, int nw, int64_t kbytes) { return kbytes >= 1024 && cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
+inline bool take_big(int64_t M, int64_t N, int nw, int64_t kbytes) { return kbytes >= 128 && cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
 
 struct WgradPlan {
   bool big;
