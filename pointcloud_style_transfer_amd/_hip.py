@@ -1470,7 +1470,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=Non
     dt = _ELEM[x.dtype]
     ws = None
     aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
-    if not aligned or D * x.element_size() % 16:
+    if M > 64 and (not aligned or D * x.element_size() % 16):
         ws = _workspace("pcst_gated_linear_workspace_size", dt, M, D, F, int(aligned), device=x.device)
     _call("pcst_gated_linear", _ptr(x), dt, M, D, _ptr(w_gate), _ptr(w_up), F, _ptr(b_gate), _ptr(b_up),
           _bias_f32(b_gate), ACTS[act], _ptr(xs), _ptr(gs), _ptr(us), _ptr(h), _ELEM[out_dtype], _ptr(ws),

@@ -548,6 +548,100 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   } while (LOOP && more);
 }
 
+// ---- few rows (M <= 64): the weights are read once, straight into the MFMA's registers.  A work-group owns
+// 16 features of both matrices; its 8 waves split k and add up in LDS, in order.  Bound by reading the weights
+// (and, at a handful of rows, by the launch).  Rows may start at any element: no copies.
+template <class E>
+__device__ __forceinline__ i32x4 piece16(const char* row, int64_t off, int64_t bytes) {
+  typedef Vec<typename E::T, 16 / elem_size<E>()> V;
+  if (off + 16 <= bytes)
+    return __builtin_bit_cast(i32x4, (typename V::V)*reinterpret_cast<const typename V::Any*>(row + off));
+  i32x4 v{0, 0, 0, 0};
+#pragma unroll
+  for (int b = 0; b < 16; b += elem_size<E>())
+    if (off + b < bytes) {
+      const uint32_t w = elem_size<E>() == 4   ? *reinterpret_cast<const uint32_t*>(row + off + b)
+                         : elem_size<E>() == 2 ? *reinterpret_cast<const uint16_t*>(row + off + b)
+                                               : *reinterpret_cast<const uint8_t*>(row + off + b);
+      v[b / 4] |= (int)(w << (8 * (b & 3)));
+    }
+  return v;
+}
+
+constexpr int kRowsMax = 64;
+
+template <class E, class O, int ACT, int TM>
+__global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
+  constexpr int ES = elem_size<E>(), P = ES == 1 ? 2 : 1, U = TM == 4 ? 2 : 4;  // pieces a product, products in flight
+  __shared__ f32x4 red[8][2][TM][64];
+  const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int f = blockIdx.x * 16 + l;
+  const int64_t bytes = g.K * ES;
+  const int steps = (int)((bytes + 64 * P - 1) / (64 * P)), per = (steps + 7) / 8;
+  const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+  const int64_t fr = f < g.N ? f : g.N - 1;  // lanes past the end repeat the last row; their results are dropped
+  const char *wg = g.b0[0] + fr * g.ldb, *wu = g.b1[0] + fr * g.ldb;
+  const char* x[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) x[i] = g.a[0] + (16 * i + l < g.M ? 16 * i + l : g.M - 1) * g.lda;
+  f32x4 acc[2][TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) acc[0][i] = acc[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = s0; s < s1; s += U) {
+    i32x4 a[U][TM][P], b[U][2][P];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int64_t off = s + u < s1 ? ((int64_t)(s + u) * P + p) * 64 + q * 16 : bytes;
+        b[u][0][p] = piece16<E>(wg, off, bytes);
+        b[u][1][p] = piece16<E>(wu, off, bytes);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) a[u][i][p] = piece16<E>(x[i], off, bytes);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if constexpr (ES == 1)
+            acc[h][i] = mma32_e4m3(a[u][i][0], a[u][i][1], b[u][h][0], b[u][h][1], acc[h][i]);
+          else
+            acc[h][i] = mma16<E>(a[u][i][0], b[u][h][0], acc[h][i]);
+        }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) red[wave][h][i][lane] = acc[h][i];
+  __syncthreads();
+  if (wave >= TM || f >= g.N) return;
+  f32x4 gv = red[0][0][wave][lane], uv = red[0][1][wave][lane];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    gv += red[w][0][wave][lane];
+    uv += red[w][1][wave][lane];
+  }
+  float bg[1], bu[1];
+  load_bias<O, 1>(g.bg, g.bias_f32, f, 1, bg);
+  load_bias<O, 1>(g.bu, g.bias_f32, f, 1, bu);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t m = 16 * wave + 4 * q + r;
+    if (m >= g.M) continue;
+    float gr = gv[r], ur = uv[r];
+    if (ES == 1) {
+      gr *= g.xs[m] * g.gs[f];
+      ur *= g.xs[m] * g.us[f];
+    }
+    gr += bg[0];
+    ur += bu[0];
+    static_cast<O*>(g.out[0])[m * g.ldo + f] = (O)(act_value<(ES < 4), ACT>(gr) * ur);
+  }
+}
+
 // ---- host side of one operand type
 struct FwdCall {
   const void *x, *wg, *wu;
@@ -645,11 +739,25 @@ inline GemmArgs fwd_args(const FwdCall& c) {
   return g;
 }
 
+template <class E, class O, int ACT>
+int launch_rows(const GemmArgs& g, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(g.N, 16));
+  if (g.M <= 16) hipLaunchKernelGGL((rows_kernel<E, O, ACT, 1>), grid, dim3(512), 0, s, g);
+  else if (g.M <= 32) hipLaunchKernelGGL((rows_kernel<E, O, ACT, 2>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((rows_kernel<E, O, ACT, 4>), grid, dim3(512), 0, s, g);
+  PCST_LAUNCH_CHECK("gated_linear");
+  return PCST_OK;
+}
+
 template <class E, class O>
 int fwd_out(const FwdCall& c, hipStream_t s) {
   GemmArgs g = fwd_args(c);
   g.out[0] = c.h;
   g.ldo = c.F;
+  if (c.M <= kRowsMax)
+    return c.act == ACT_SILU   ? launch_rows<E, O, ACT_SILU>(g, s)
+           : c.act == ACT_GELU ? launch_rows<E, O, ACT_GELU>(g, s)
+                               : launch_rows<E, O, ACT_RELU>(g, s);
   return launch_gated<E, O, EPI_FWD>(g, s, c.act);
 }
 

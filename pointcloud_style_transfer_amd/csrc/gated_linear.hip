@@ -102,7 +102,7 @@ extern "C" int pcst_gated_linear_workspace_size(int dtype, int64_t M, int64_t D,
                                                 size_t* bytes) {
   if (int rc = check("gated_linear_workspace_size", dtype, M, D, F, 0)) return rc;
   PCST_CHECK_ARG(bytes, "gated_linear_workspace_size: null pointer");
-  *bytes = aligned && (D * elem(dtype)) % 16 == 0 ? 0 : lay(nullptr, dtype, M, D, F, false).bytes;
+  *bytes = M <= gated::kRowsMax || (aligned && (D * elem(dtype)) % 16 == 0) ? 0 : lay(nullptr, dtype, M, D, F, false).bytes;
   return PCST_OK;
 }
 
@@ -122,13 +122,21 @@ extern "C" int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D,
   if (M == 0) return PCST_OK;
   PCST_CHECK_ARG(x && w_gate && w_up && h, "gated_linear: null pointer");
   const int es = elem(dtype);
-  const bool direct = ready(x, D, es) && ready(w_gate, D, es) && ready(w_up, D, es);
+  const bool rows = M <= gated::kRowsMax;
+  const bool direct = rows || (ready(x, D, es) && ready(w_gate, D, es) && ready(w_up, D, es));
   PCST_CHECK_ARG(direct || workspace, "gated_linear: rows off 16-byte boundaries need the workspace");
   gated::FwdCall c{};
   c.M = M;
   c.D = D;
   c.F = F;
-  operands(c, lay(workspace, dtype, M, D, F, false), x, w_gate, w_up, es, as_stream(stream));
+  if (rows) {
+    c.x = x;
+    c.wg = w_gate;
+    c.wu = w_up;
+    c.ldx = c.ldw = D * es;
+  } else {
+    operands(c, lay(workspace, dtype, M, D, F, false), x, w_gate, w_up, es, as_stream(stream));
+  }
   c.bg = b_gate;
   c.bu = b_up;
   c.bias_f32 = bias_f32;
