@@ -8,8 +8,10 @@ CPU tensor is an error.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import operator
 import os
 
 import numpy as np
@@ -1331,6 +1333,17 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 ACTS = {"silu": 0, "gelu": 1, "relu": 2}
 
 
+# Serving calls these for a few rows at a time, where the host's share of a call is what is waited for:
+# addresses and the stream go to ctypes as plain integers (torch.cuda.current_stream() builds a Stream
+# object, 2.8 us a call; the raw handle 0.1 us).
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream():
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _same_device(what, t, *others):
     require_device(t, *others)
     d = t.get_device()
@@ -1367,8 +1380,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, stats=False):
     y = torch.empty_like(x)
     s = x if residual is None else torch.empty_like(x)
     rho = torch.empty(M, dtype=torch.float32, device=x.device) if stats else None
-    _call("pcst_rms_norm", _ptr(x), _ptr(residual), _ELEM[x.dtype], M, D, _ptr(weight),
-          _ELEM[weight.dtype], eps, _ptr(y), _ptr(s), _ptr(rho), _stream())
+    _call("pcst_rms_norm", _addr(x), _addr(residual), _ELEM[x.dtype], M, D, _addr(weight),
+          _ELEM[weight.dtype], eps, _addr(y), _addr(s), _addr(rho), _raw_stream())
     return y, s, rho
 
 
@@ -1387,8 +1400,8 @@ def rms_norm_bwd(s, weight, rho, dy, ds=None, need_dx=True, need_dw=True):
     dx = torch.empty_like(s) if need_dx else None
     dw = torch.empty_like(weight) if need_dw else None
     ws = _workspace("pcst_rms_norm_bwd_workspace_size", M, D, device=s.device) if need_dw else None
-    _call("pcst_rms_norm_bwd", _ptr(s), _ELEM[s.dtype], M, D, _ptr(weight), _ELEM[weight.dtype],
-          _ptr(rho), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw), _ptr(ws), _stream())
+    _call("pcst_rms_norm_bwd", _addr(s), _ELEM[s.dtype], M, D, _addr(weight), _ELEM[weight.dtype],
+          _addr(rho), _addr(dy), _addr(ds), _addr(dx), _addr(dw), _addr(ws), _raw_stream())
     return dx, dw
 
 
@@ -1399,8 +1412,8 @@ def rms_norm_quant(x, weight, residual=None, eps=1e-6):
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     s = x if residual is None else torch.empty_like(x)
-    _call("pcst_rms_norm_quant", _ptr(x), _ptr(residual), _ELEM[x.dtype], M, D, _ptr(weight),
-          _ELEM[weight.dtype], eps, _ptr(q), _ptr(scale), _ptr(s), _stream())
+    _call("pcst_rms_norm_quant", _addr(x), _addr(residual), _ELEM[x.dtype], M, D, _addr(weight),
+          _ELEM[weight.dtype], eps, _addr(q), _addr(scale), _addr(s), _raw_stream())
     return q, scale, s
 
 
@@ -1410,7 +1423,7 @@ def quant_rows(x):
     x, _, _, M, D = _norm_operands("quant_rows", x, None, None)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call("pcst_quant_rows", _ptr(x), _ELEM[x.dtype], M, D, _ptr(q), _ptr(scale), _stream())
+    _call("pcst_quant_rows", _addr(x), _ELEM[x.dtype], M, D, _addr(q), _addr(scale), _raw_stream())
     return q, scale
 
 
@@ -1472,9 +1485,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=Non
     aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
     if M > 64 and (not aligned or D * x.element_size() % 16):
         ws = _workspace("pcst_gated_linear_workspace_size", dt, M, D, F, int(aligned), device=x.device)
-    _call("pcst_gated_linear", _ptr(x), dt, M, D, _ptr(w_gate), _ptr(w_up), F, _ptr(b_gate), _ptr(b_up),
-          _bias_f32(b_gate), ACTS[act], _ptr(xs), _ptr(gs), _ptr(us), _ptr(h), _ELEM[out_dtype], _ptr(ws),
-          _stream())
+    _call("pcst_gated_linear", _addr(x), dt, M, D, _addr(w_gate), _addr(w_up), F, _addr(b_gate), _addr(b_up),
+          _bias_f32(b_gate), ACTS[act], _addr(xs), _addr(gs), _addr(us), _addr(h), _ELEM[out_dtype], _addr(ws),
+          _raw_stream())
     return h
 
 
@@ -1502,17 +1515,17 @@ def gated_linear_bwd(x, w_gate, w_up, dh, b_gate=None, b_up=None, act="silu", ne
     if M and any(t is not None for t in [dx, *dw, *db]):
         dt = _ELEM[x.dtype]
         ws = _workspace("pcst_gated_linear_bwd_workspace_size", dt, M, D, F, device=dev)
-        _call("pcst_gated_linear_bwd", _ptr(x), dt, M, D, _ptr(w_gate), _ptr(w_up), F, _ptr(b_gate),
-              _ptr(b_up), _bias_f32(b_gate), ACTS[act], _ptr(dh), _ptr(dx), _ptr(dw[0]), _ptr(dw[1]),
-              1 if wgrad_dtype == torch.float32 else 0, _ptr(db[0]), _ptr(db[1]), _ptr(ws), _stream())
+        _call("pcst_gated_linear_bwd", _addr(x), dt, M, D, _addr(w_gate), _addr(w_up), F, _addr(b_gate),
+              _addr(b_up), _bias_f32(b_gate), ACTS[act], _addr(dh), _addr(dx), _addr(dw[0]), _addr(dw[1]),
+              1 if wgrad_dtype == torch.float32 else 0, _addr(db[0]), _addr(db[1]), _addr(ws), _raw_stream())
     return (dx, *dw, *db)
 
 
 # ----------------------------------------------------------------------------- gradient clipping
 def _dense(t):
     """Whether t's elements fill its memory without gaps, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
+    if t.layout != torch.strided:
+        return False
     n = 1
     for size, stride in sorted(((a, b) for a, b in zip(t.shape, t.stride()) if a != 1), key=lambda p: p[1]):
         if stride != n:
@@ -1522,14 +1535,52 @@ def _dense(t):
 
 
 _NORM_P = {1.0: 1, 2.0: 2, float("inf"): 0}
+# a method or attribute of every tensor of a list, without a Python frame for each
+_T = torch.Tensor
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _clip_lists(grads, out):
+    """(addresses, sizes, type codes) of the tensors and the outputs' (addresses, type codes), as C arrays:
+    array.array and bytes.  Checks types, devices and layouts."""
+    n = len(grads)
+    both = grads if out is None else grads + out
+    dtypes = list(map(_dtype_of, both))
+    if not set(dtypes) <= set(_FLOATS):
+        raise RuntimeError(f"grad_clip: dense float32, bfloat16 or float16 tensors only, got "
+                           f"{[d for d in set(dtypes) if d not in _FLOATS]}")
+    if not all(map(_T.is_contiguous, both)):
+        for i, t in enumerate(both):
+            if not _dense(t):
+                raise RuntimeError(f"grad_clip: a tensor with gaps (strides {t.stride()} of {list(t.shape)}); "
+                                   "pass its contiguous copy")
+            g = grads[i % n]
+            if not (t.is_contiguous() and g.is_contiguous()) and (t.shape != g.shape or t.stride() != g.stride()):
+                raise RuntimeError("grad_clip: an output has its gradient's strides unless both are contiguous")
+    numel = array.array("q", map(_T.numel, grads))
+    elem = bytes(map(_ELEM.__getitem__, dtypes))
+    types = elem[:n]
+    if out is not None:
+        if numel != array.array("q", map(_T.numel, out)) or any(
+                o != g and o != torch.float32 for g, o in zip(dtypes, dtypes[n:])):
+            raise RuntimeError("grad_clip: an output has its gradient's number of elements, and its type or float32")
+        types = bytes(a | b << 4 for a, b in zip(types, elem[n:]))
+    else:
+        types = bytes(a * 17 for a in types)  # the same type twice
+    devices = set(map(_T.get_device, both))
+    if len(devices) > 1 or -1 in devices:
+        require_device(*both)
+        raise RuntimeError("grad_clip: tensors on different devices")
+    ptr = array.array("q", map(_T.data_ptr, grads))
+    return ptr, numel, types, ptr if out is None else array.array("q", map(_T.data_ptr, out))
 
 
 def grad_clip(grads, max_norm, norm_type=2.0, inv_scale=None, out=None, scale=True):
     """The norm of all `grads` together (times inv_scale, a float32 device tensor of one element) ->
     float32 tensor []; with scale, out[i] = grads[i] * inv_scale * min(1, max_norm / (norm + 1e-6)),
     out None: in place.  grads: dense tensors of float32, bfloat16 or float16 on one device, no two of
-    them (or of the outputs) overlapping; out[i] like grads[i] in shape and strides, of its type or
-    float32.  norm_type 1, 2 or inf.  Nothing waits for the device."""
+    them (or of the outputs) overlapping; out[i] contiguous like grads[i] with as many elements, or of its
+    strides, of its type or float32.  norm_type 1, 2 or inf.  Nothing waits for the device."""
     grads = list(grads)
     p = _NORM_P.get(float(norm_type))
     if p is None:
@@ -1544,49 +1595,18 @@ def grad_clip(grads, max_norm, norm_type=2.0, inv_scale=None, out=None, scale=Tr
         out = list(out)
         if len(out) != n:
             raise RuntimeError(f"grad_clip: {len(out)} outputs for {n} gradients")
-    dev = grads[0].get_device()
-    for t in grads if out is None else grads + out:
-        if t.dtype not in _FLOATS or t.layout != torch.strided:
-            raise RuntimeError(f"grad_clip: dense float32, bfloat16 or float16 tensors only, got {t.dtype} "
-                               f"({t.layout})")
-        if not (t.is_contiguous() or _dense(t)):
-            raise RuntimeError(f"grad_clip: a tensor with gaps (strides {t.stride()} of {list(t.shape)}); "
-                               "pass its contiguous copy")
-    ptr = np.fromiter([t.data_ptr() for t in grads], np.int64, n)
-    numel = np.fromiter([t.numel() for t in grads], np.int64, n)
-    elem = np.fromiter([_ELEM[t.dtype] for t in grads], np.uint8, n)
-    lo, hi = ptr, ptr + numel * np.where(elem == 0, 4, 2)
-    optr, oelem = ptr, elem
-    if out is not None:
-        for g, o in zip(grads, out):
-            if o.shape != g.shape or not (o.dtype == g.dtype or o.dtype == torch.float32) \
-                    or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise RuntimeError("grad_clip: an output has its gradient's shape and strides, and its type "
-                                   f"or float32; got {o.dtype} {list(o.shape)} for {g.dtype} {list(g.shape)}")
-        optr = np.fromiter([t.data_ptr() for t in out], np.int64, n)
-        oelem = np.fromiter([_ELEM[t.dtype] for t in out], np.uint8, n)
-        other = (optr != ptr) | (oelem != elem)
-        lo = np.concatenate([lo, optr[other]])
-        hi = np.concatenate([hi, (optr + numel * np.where(oelem == 0, 4, 2))[other]])
-    some = hi > lo
-    lo, hi = lo[some], hi[some]
-    order = np.argsort(lo)
-    if bool((lo[order][1:] < hi[order][:-1]).any()):
-        raise RuntimeError("grad_clip: two of the tensors overlap (or one is given twice)")
+    ptr, numel, types, optr = _clip_lists(grads, out)
+    dev = grads[0].device
     if inv_scale is not None and (inv_scale.dtype != torch.float32 or inv_scale.numel() != 1
-                                  or inv_scale.get_device() != dev):
+                                  or inv_scale.device != dev):
         raise RuntimeError("grad_clip: inv_scale is one float32 on the gradients' device")
-    if dev < 0 or any(t.get_device() != dev for t in (grads if out is None else grads + out)):
-        require_device(*grads)
-        raise RuntimeError("grad_clip: tensors on different devices")
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    types = elem | (oelem << 4)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    sizes = numel.buffer_info()[0]
     sz = ctypes.c_size_t(0)
-    np_ptr = lambda a: ctypes.c_void_p(a.ctypes.data)  # noqa: E731
-    _call("pcst_grad_clip_workspace_size", np_ptr(numel), n, ctypes.byref(sz))
-    ws = torch.empty(sz.value, dtype=torch.uint8, device=norm.device)
-    _call("pcst_grad_clip", np_ptr(ptr), np_ptr(optr) if scale else None, np_ptr(numel), np_ptr(types), n, p,
-          max_norm, _ptr(inv_scale), _ptr(norm), _ptr(ws), _stream())
+    _call("pcst_grad_clip_workspace_size", sizes, n, ctypes.byref(sz))
+    ws = torch.empty(sz.value, dtype=torch.uint8, device=dev)
+    _call("pcst_grad_clip", ptr.buffer_info()[0], optr.buffer_info()[0] if scale else None, sizes, types, n, p,
+          max_norm, _addr(inv_scale), norm.data_ptr(), ws.data_ptr(), _raw_stream())
     if scale:  # what autograd saved of these tensors is now another value
         torch.autograd.graph.increment_version(grads if out is None else out)
     return norm

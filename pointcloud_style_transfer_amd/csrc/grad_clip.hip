@@ -9,6 +9,10 @@
 // between.  fp64 sums: a square of any finite float is finite there, and the order does not show in the
 // 24 bits returned.  The tensors' addresses travel in the kernel arguments, so a captured launch keeps
 // them.  Bound by HBM: every gradient is read twice and written once.
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "ops_types.h"
 
 namespace pcst {
@@ -181,6 +185,25 @@ __global__ __launch_bounds__(256) void grad_total_kernel(const double* __restric
   if (threadIdx.x == 0) *norm = (float)((p == 2 ? sqrt(s) : s) * fabs(inv_scale ? (double)*inv_scale : 1.0));
 }
 
+// whether two of the tensors' byte ranges overlap (a gradient written in place counts once)
+bool overlap(const void* const* in, void* const* out, const int64_t* n, const uint8_t* type, int count) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> r;
+  r.reserve(2 * (size_t)count);
+  auto add = [&](const void* p, int64_t len, int t) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    r.emplace_back(a, a + (uintptr_t)len * (t == kF32 ? 4 : 2));
+  };
+  for (int i = 0; i < count; ++i) {
+    if (n[i] == 0) continue;
+    add(in[i], n[i], type[i] & 15);
+    if (out && (out[i] != in[i] || (type[i] & 15) != type[i] >> 4)) add(out[i], n[i], type[i] >> 4);
+  }
+  std::sort(r.begin(), r.end());
+  for (size_t i = 1; i < r.size(); ++i)
+    if (r[i].first < r[i - 1].second) return true;
+  return false;
+}
+
 bool is_float(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 
 }  // namespace
@@ -209,6 +232,14 @@ extern "C" int pcst_grad_clip(const void* const* grads, void* const* out, const 
   }
   const int64_t total = clip_total(numel, count);
   PCST_CHECK_ARG(total < (1ll << 40), "grad_clip: too many elements");
+  bool clash = false;
+  try {
+    clash = overlap(grads, out, numel, types, count);
+  } catch (...) {  // nothing is thrown across the C boundary
+    set_error("grad_clip: no host memory for %d tensors", count);
+    return PCST_EINVAL;
+  }
+  PCST_CHECK_ARG(!clash, "grad_clip: two of the tensors overlap (or one is given twice)");
   hipStream_t s = as_stream(stream);
   PCST_CHECK_ARG(total == 0 || workspace, "grad_clip: null workspace");
   double* part = static_cast<double*>(workspace);

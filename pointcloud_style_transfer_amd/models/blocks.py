@@ -16,8 +16,12 @@ from .. import _hip
 from . import _autograd as _ag
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _no_grad_form(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _wants_grad(*tensors):
         raise RuntimeError(f"{name}: no gradients flow through 8 bits; call it under torch.no_grad()")
 
 
@@ -25,7 +29,10 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     """Root-mean-square norm over the last dimension (at most 16384 wide) -> y like x, or with a
     residual (y, s), s = x + residual rounded to x's type and y its norm.  x float32, bfloat16 or
     float16; weight [D] of x's type or float32.  Differentiable in x, weight and residual."""
-    return _ag.RMSNormFn.apply(x, weight, residual, float(eps))
+    if _wants_grad(x, weight, residual):
+        return _ag.RMSNormFn.apply(x, weight, residual, float(eps))
+    y, s, _ = _hip.rms_norm(x, weight, residual, float(eps))
+    return y if residual is None else (y, s)
 
 
 def rms_norm_quant(x, weight, residual=None, eps=1e-6):
@@ -47,7 +54,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up), x [..., D], weights [F, D] -> [..., F], in one
     kernel.  Operands of one type (float32, bfloat16 or float16; under torch.autocast they are rounded
     to its type), biases of that type or float32; act "silu", "gelu" or "relu".  Differentiable."""
-    return _ag.GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, act)
+    if (x.dim() != 2 or torch.is_autocast_enabled("cuda") or _wants_grad(x, w_gate, w_up, b_gate, b_up)):
+        return _ag.GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, act)
+    return _hip.gated_linear(x, w_gate, w_up, b_gate, b_up, act)
 
 
 def gated_linear_quant(q, scale, w_gate, gate_scale, w_up, up_scale, b_gate=None, b_up=None, act="silu",

@@ -129,6 +129,8 @@ def z(*shape, dtype=BF):
     (lambda: _hip.grad_clip([z(4)], 1.0, out=[z(5)]), "an output has"),
     (lambda: _hip.grad_clip([z(4)], 1.0, out=[z(4, dtype=torch.float16)]), "an output has"),
     (lambda: _hip.grad_clip([z(4, 4)], 1.0, out=[z(4, 4).t()]), "an output has"),
+    (lambda: _hip.grad_clip([z(4, 4).t()], 1.0, out=[z(4, 4)]), "an output has"),
+    (lambda: _hip.grad_clip([z(4, 4).t()], 1.0, out=[z(2, 8).t()]), "an output has"),
     (lambda: _hip.grad_clip([z(4, dtype=torch.float64)], 1.0), "dense float32"),
     (lambda: _hip.grad_clip([z(4, 8)[:, ::2]], 1.0), "gaps"),
     (lambda: _hip.grad_clip([z(1, 8).expand(4, 8)], 1.0), "gaps"),
@@ -139,16 +141,31 @@ def test_binding_refusals(call, match):
         call()
 
 
+def clip_rc(grads, out):
+    """pcst_grad_clip on host addresses and without a workspace: refused for one or for the other."""
+    n = len(grads)
+    P, I, U = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_uint8 * n
+    code = lambda t: _hip._ELEM[t.dtype]  # noqa: E731
+    outs = grads if out is None else out
+    one = ctypes.c_void_p(16)
+    lib_args = (P(*[t.data_ptr() for t in grads]), P(*[t.data_ptr() for t in outs]), I(*[t.numel() for t in grads]),
+                U(*[code(g) | code(o) << 4 for g, o in zip(grads, outs)]), n, 2, 1.0, None, one, None, None)
+    assert rc("pcst_grad_clip", *lib_args) == EINVAL
+    return error()
+
+
 def test_clip_refuses_overlap():
-    a = z(32)
-    for grads, out in (([a, a], None), ([a[:20], a[16:]], None), ([a[:8]], [a[4:12]]), ([a[:8], a[8:16]], [z(8), a[:8]])):
-        with pytest.raises(RuntimeError, match="overlap"):
-            _hip.grad_clip(grads, 1.0, out=out)
-    # neighbours in one buffer, a gradient onto itself, empty tensors and dense permutations are fine
-    b = z(4, 6, 5).permute(2, 0, 1)
-    for grads, out in (([a[:16], a[16:]], None), ([a[:8]], [a[:8]]), ([a, a[:0], a[8:8]], None), ([b], None), ([b], [b])):
+    a, f = z(32), z(32, dtype=F32)
+    for grads, out in (([a, a], None), ([a[:20], a[16:]], None), ([a[:8]], [a[4:12]]), ([a[:8], a[8:16]], [z(8), a[:8]]),
+                       ([f.view(BF)[:32]], [f])):
+        assert "overlap" in clip_rc(grads, out)
+    # neighbours in one buffer, a gradient onto itself and empty tensors are fine
+    for grads, out in (([a[:16], a[16:]], None), ([a[:8]], [a[:8]]), ([a, a[:0], a[8:8]], None), ([a[:8]], [f[:8]])):
+        assert "workspace" in clip_rc(grads, out)
+    b = z(4, 6, 5).permute(2, 0, 1)  # dense, in another order
+    for out in (None, [b], [torch.empty_like(b)]):
         with pytest.raises(RuntimeError, match="HIP device"):
-            _hip.grad_clip(grads, 1.0, out=out)
+            _hip.grad_clip([b], 1.0, out=out)
 
 
 def test_eight_bits_carry_no_gradients():
