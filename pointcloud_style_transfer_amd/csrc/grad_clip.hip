@@ -5,8 +5,7 @@
 //
 // Two launches (per 128 tensors): the norm's, whose work-groups each leave one partial in fp64, and
 // the scaling's, whose work-groups each add all partials in the same fixed order themselves -- at most
-// 1024 + (number of tensors) of them, so that no third launch, no atomic and no zeroed counter stands
-// between.  fp64 sums: a square of any finite float is finite there, and the order does not show in the
+// 1024 a launch, so that no third launch, no atomic and no zeroed counter stands between.  fp64 sums: a square of any finite float is finite there, and the order does not show in the
 // 24 bits returned.  The tensors' addresses travel in the kernel arguments, so a captured launch keeps
 // them.  Bound by HBM: every gradient is read twice and written once.
 #include <algorithm>
@@ -62,18 +61,31 @@ __device__ __forceinline__ double block_total(double v, int p, double* red) {
   return s;
 }
 
+__device__ __forceinline__ double add_term(double s, float v, int p) {
+  const double d = (double)v;
+  return p == 2 ? fma(d, d, s) : p == 1 ? s + fabs(d) : nan_max(s, fabs(d));
+}
+
+constexpr int kFlight = 4;  // 8-value pieces a thread has in flight
+
 template <class T>
-__device__ __forceinline__ double range_sum(const T* g, int64_t lo, int64_t hi, int p) {
-  double s = 0.0;
-#pragma unroll 2
-  for (int64_t i = lo + threadIdx.x * 8; i < hi; i += 256 * 8) {
-    float v[8];
-    load8(g + i, (int)(hi - i < 8 ? hi - i : 8), v);
+__device__ __forceinline__ double range_sum(const T* g, int64_t lo, int64_t hi, int p, double s) {
+  typedef typename Vec<T, 8>::V V;
+  int64_t i = lo + threadIdx.x * 8;
+  for (; i + (kFlight - 1) * 2048 + 8 <= hi; i += kFlight * 2048) {
+    V v[kFlight];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double d = (double)v[j];
-      s = p == 2 ? fma(d, d, s) : p == 1 ? s + fabs(d) : nan_max(s, fabs(d));
-    }
+    for (int u = 0; u < kFlight; ++u) v[u] = *reinterpret_cast<const typename Vec<T, 8>::Any*>(g + i + u * 2048);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = add_term(s, (float)v[u][j], p);
+  }
+  for (; i < hi; i += 2048) {
+    float v[8];
+    load8(g + i, (int)(hi - i < 8 ? hi - i : 8), v);  // zeros past the end add nothing
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = add_term(s, v[j], p);
   }
   return s;
 }
@@ -81,22 +93,37 @@ __device__ __forceinline__ double range_sum(const T* g, int64_t lo, int64_t hi, 
 __global__ __launch_bounds__(256) void grad_norm_kernel(ClipTable t, int64_t chunk_len, int p,
                                                         double* __restrict__ part) {
   __shared__ double red[4];
-  const int k = find_tensor(t, blockIdx.x);
-  const int64_t lo = (int64_t)(blockIdx.x - t.first[k]) * chunk_len;
-  const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
-  const int type = t.type[k] & 15;
-  double s;
-  if (type == kF32) s = range_sum(static_cast<const float*>(t.in[k]), lo, hi, p);
-  else if (type == kBF16) s = range_sum(static_cast<const __bf16*>(t.in[k]), lo, hi, p);
-  else s = range_sum(static_cast<const _Float16*>(t.in[k]), lo, hi, p);
+  double s = 0.0;
+  for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+    const int k = find_tensor(t, c);
+    const int64_t lo = (int64_t)(c - t.first[k]) * chunk_len;
+    const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
+    const int type = t.type[k] & 15;
+    if (type == kF32) s = range_sum(static_cast<const float*>(t.in[k]), lo, hi, p, s);
+    else if (type == kBF16) s = range_sum(static_cast<const __bf16*>(t.in[k]), lo, hi, p, s);
+    else s = range_sum(static_cast<const _Float16*>(t.in[k]), lo, hi, p, s);
+  }
   s = block_total(s, p, red);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
 template <class T, class O>
 __device__ __forceinline__ void range_scale(const T* g, O* o, int64_t lo, int64_t hi, float f) {
-#pragma unroll 2
-  for (int64_t i = lo + threadIdx.x * 8; i < hi; i += 256 * 8) {
+  typedef typename Vec<T, 8>::V V;
+  int64_t i = lo + threadIdx.x * 8;
+  for (; i + (kFlight - 1) * 2048 + 8 <= hi; i += kFlight * 2048) {
+    V v[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) v[u] = *reinterpret_cast<const typename Vec<T, 8>::Any*>(g + i + u * 2048);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = (float)v[u][j] * f;
+      store8(o + i + u * 2048, 8, w);
+    }
+  }
+  for (; i < hi; i += 2048) {
     const int n = (int)(hi - i < 8 ? hi - i : 8);
     float v[8];
     load8(g + i, n, v);
@@ -118,26 +145,34 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(ClipTable t, int64_t ch
   const double inv = inv_scale ? (double)*inv_scale : 1.0;
   const double total = (p == 2 ? sqrt(s) : s) * fabs(inv);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
-  double c = max_norm / (total + 1e-6);
-  c = c > 1.0 ? 1.0 : c;  // NaN stays
-  const float f = (float)(c * inv);
-  const int k = find_tensor(t, blockIdx.x);
-  if (f == 1.0f && t.in[k] == t.out[k]) return;  // g * 1 is g
-  const int64_t lo = (int64_t)(blockIdx.x - t.first[k]) * chunk_len;
-  const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
-  const void* g = t.in[k];
-  void* o = t.out[k];
-  switch (t.type[k]) {
-    case kF32 | kF32 << 4: range_scale(static_cast<const float*>(g), static_cast<float*>(o), lo, hi, f); break;
-    case kBF16 | kBF16 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<__bf16*>(o), lo, hi, f); break;
-    case kF16 | kF16 << 4: range_scale(static_cast<const _Float16*>(g), static_cast<_Float16*>(o), lo, hi, f); break;
-    case kBF16 | kF32 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<float*>(o), lo, hi, f); break;
-    default: range_scale(static_cast<const _Float16*>(g), static_cast<float*>(o), lo, hi, f); break;
+  double q = max_norm / (total + 1e-6);
+  q = q > 1.0 ? 1.0 : q;  // NaN stays
+  const float f = (float)(q * inv);
+  // from the last chunk down: what the norm's launch read last is still in the caches
+  for (int b = blockIdx.x; b < t.first[t.count]; b += gridDim.x) {
+    const int c = t.first[t.count] - 1 - b;
+    const int k = find_tensor(t, c);
+    if (f == 1.0f && t.in[k] == t.out[k]) continue;  // g * 1 is g
+    const int64_t lo = (int64_t)(c - t.first[k]) * chunk_len;
+    const int64_t hi = lo + chunk_len < t.n[k] ? lo + chunk_len : t.n[k];
+    const void* g = t.in[k];
+    void* o = t.out[k];
+    switch (t.type[k]) {
+      case kF32 | kF32 << 4: range_scale(static_cast<const float*>(g), static_cast<float*>(o), lo, hi, f); break;
+      case kBF16 | kBF16 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<__bf16*>(o), lo, hi, f); break;
+      case kF16 | kF16 << 4: range_scale(static_cast<const _Float16*>(g), static_cast<_Float16*>(o), lo, hi, f); break;
+      case kBF16 | kF32 << 4: range_scale(static_cast<const __bf16*>(g), static_cast<float*>(o), lo, hi, f); break;
+      default: range_scale(static_cast<const _Float16*>(g), static_cast<float*>(o), lo, hi, f); break;
+    }
   }
 }
 
-// elements per work-group: about 1024 work-groups over all tensors, at least 2048 elements each
-int64_t clip_chunk(int64_t total) { return std::max<int64_t>(2048, cdiv(cdiv(total, 1024), 2048) * 2048); }
+// A chunk is what a work-group takes at a time; a launch has at most kClipGroups work-groups (4 a CU, each
+// thread with kFlight loads in flight), which take chunk after chunk and leave one partial each.
+constexpr int kClipGroups = 1024;
+int64_t clip_chunk(int64_t total) {
+  return std::max<int64_t>(2048, std::min<int64_t>(65536, cdiv(cdiv(total, kClipGroups), 2048) * 2048));
+}
 
 int64_t clip_total(const int64_t* n, int count) {
   int64_t t = 0;
@@ -145,10 +180,20 @@ int64_t clip_total(const int64_t* n, int count) {
   return t;
 }
 
+// partials of all launches
 int64_t clip_parts(const int64_t* n, int count, int64_t chunk) {
-  int64_t t = 0;
-  for (int i = 0; i < count; ++i) t += cdiv(n[i], chunk);
-  return t;
+  int64_t parts = 0, c = 0;
+  int in = 0;
+  for (int i = 0; i < count; ++i) {
+    if (n[i] == 0) continue;
+    c += cdiv(n[i], chunk);
+    if (++in == kClipTensors) {
+      parts += std::min<int64_t>(c, kClipGroups);
+      in = 0;
+      c = 0;
+    }
+  }
+  return parts + std::min<int64_t>(c, kClipGroups);
 }
 
 template <class F>
@@ -170,8 +215,9 @@ void for_tables(const void* const* in, void* const* out, const int64_t* n, const
     }
     if (t.count == 0) break;
     t.first[t.count] = c;
-    f(t, c, base);
-    base += c;
+    const int32_t groups = std::min<int32_t>(c, kClipGroups);
+    f(t, groups, base);
+    base += groups;
   }
 }
 

@@ -19,7 +19,9 @@ namespace pcst {
 namespace {
 
 constexpr int kNormMaxD = 16384;
-constexpr int kNormMaxParts = 512;  // partial rows of dw
+// partial rows of dw: enough work-groups to keep HBM busy, few enough that the partials stay small next to
+// the operands (4 bytes a column each, written and read once)
+constexpr int kNormParts = 512, kNormPartsNarrow = 2048, kNormNarrow = 512;
 
 template <int TPR>
 __device__ __forceinline__ float row_reduce(float v, bool maximum, float* red) {
@@ -129,13 +131,20 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(NormArg
         for (int k = 0; k < 8; ++k) top = c0 + i * TPR * 8 + k < D ? fmaxf(top, fabsf(v[i][k])) : top;
       top = row_reduce<TPR>(top, true, red);
       const float sc = top > 0.0f ? top / 448.0f : 1.0f;
+      const float inv = 1.0f / sc;
+      const bool plain = !(sc > 0x1p-100f && sc < 0x1p100f);
       if (live && lane == 0) a.scale[row] = sc;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = c0 + i * TPR * 8, n = D - c;
         if (n <= 0 || !live) continue;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] / sc;
+        for (int k = 0; k < 8; ++k) {
+          // the quotient from the reciprocal and one correction; the division itself for scales whose
+          // reciprocal is no normal number
+          const float q0 = v[i][k] * inv;
+          v[i][k] = plain ? v[i][k] / sc : fmaf(fmaf(-q0, sc, v[i][k]), inv, q0);
+        }
         const uint2 q = pack8_e4m3(v[i]);
         uint8_t* out = static_cast<uint8_t*>(a.y) + at + c;
         if (n >= 8) {
@@ -167,10 +176,24 @@ struct NormBwdArgs {
   float* part;  // [gridDim.x, D] or null
 };
 
+// 8 values as they are stored, the first n of them, zeros behind
+template <class T>
+__device__ __forceinline__ typename Vec<T, 8>::V raw8(const T* p, int n) {
+  if (n >= 8) return *reinterpret_cast<const typename Vec<T, 8>::Any*>(p);
+  typename Vec<T, 8>::V v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+  return v;
+}
+
+// One row of s, dy and ds in flight while the previous one is worked on: with few work-groups (each
+// leaves a partial row of dw) the loads of one row at a time keep too little of HBM busy.
 template <class T, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(NormBwdArgs a) {
+  typedef typename Vec<T, 8>::V V;
   constexpr int kThreads = TPR > 256 ? TPR : 256;
   constexpr int RPB = kThreads / TPR;
+  constexpr bool AHEAD = NV < 4;  // (the widest rows have no registers left for it)
   __shared__ float red[8];
   __shared__ float cs[RPB > 1 ? TPR * NV * 8 : 1];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -184,48 +207,55 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(NormBwd
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[i][k] = 0.0f;
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.M; row0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = row0 + sub;
-    const bool live = row < a.M;
-    const int64_t at = (live ? row : row0) * D;
-    const float rho = live ? a.rho[row] : 0.0f;
-    float n_[NV][8], g[NV][8];
-    float dot = 0.0f;
+  V sv[NV], gv[NV], dv[NV];
+  float rho = 0.0f;
+  auto fetch = [&](int64_t row, bool live) {
+    rho = live ? a.rho[row] : 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = c0 + i * TPR * 8, n = D - c;
-      if (n > 0) {
-        load8(sp + at + c, n, n_[i]);
-        load8(dyp + at + c, n, g[i]);
-      } else {
+      const int c = c0 + i * TPR * 8, n = live ? D - c : 0;
+      const int64_t at = row * D + c;
+      sv[i] = n > 0 ? raw8(sp + at, n) : V{};
+      gv[i] = n > 0 ? raw8(dyp + at, n) : V{};
+      dv[i] = n > 0 && dsp ? raw8(dsp + at, n) : V{};
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + sub;
+  if (AHEAD) fetch(row, row < a.M);
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.M; row0 += step, row += step) {
+    const bool live = row < a.M;
+    if (!AHEAD) fetch(row, live);
+    float n_[NV][8], g[NV][8], o[NV][8];
+    float dot = 0.0f;
+    const float r = rho;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) n_[i][k] = g[i][k] = 0.0f;
-      }
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        n_[i][k] *= rho;
-        if (live) acc[i][k] = fmaf(g[i][k], n_[i][k], acc[i][k]);
+        n_[i][k] = (float)sv[i][k] * r;
+        g[i][k] = (float)gv[i][k];
+        o[i][k] = (float)dv[i][k];
+      }
+    if (AHEAD && row0 + step < a.M) fetch(row + step, row + step < a.M);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // (a row past the end is all zeros)
+        acc[i][k] = fmaf(g[i][k], n_[i][k], acc[i][k]);
         g[i][k] *= wv[i][k];
         dot = fmaf(g[i][k], n_[i][k], dot);
       }
-    }
+    if (!a.dx) continue;
     const float c1 = row_reduce<TPR>(dot, false, red) / (float)D;
-    if (!live || !a.dx) continue;  // (live is the same for every thread of a row; row_reduce's
-                                   //  barriers run only where a row is the whole work-group)
+    if (!live) continue;  // (no barrier is skipped: more than one row a work-group means none is used)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = c0 + i * TPR * 8, n = D - c;
       if (n <= 0) continue;
-      float o[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = rho * (g[i][k] - n_[i][k] * c1);
-      if (dsp) {
-        float t[8];
-        load8(dsp + at + c, n, t);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] += t[k];
-      }
-      store8(static_cast<T*>(a.dx) + at + c, n, o);
+      for (int k = 0; k < 8; ++k) o[i][k] += r * (g[i][k] - n_[i][k] * c1);
+      store8(static_cast<T*>(a.dx) + row * D + c, n, o[i]);
     }
   }
   if (!a.part) return;
@@ -253,21 +283,27 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(NormBwd
   }
 }
 
-// dw[d] = sum over the partial rows, 16 columns a work-group, 16 slices of the rows, fp64, in order
-__global__ __launch_bounds__(256) void norm_dw_kernel(const float* __restrict__ part, int parts, int D,
-                                                      void* dw, int dwt) {
-  __shared__ double red[16][17];
+// dw[d] = sum over the partial rows, 16 columns a work-group, 64 slices of the rows, fp64, in a fixed order
+__global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int parts, int D,
+                                                       void* dw, int dwt) {
+  __shared__ double red[64][17];
   const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int d = blockIdx.x * 16 + c;
   double s = 0.0;
   if (d < D) {
 #pragma unroll 8
-    for (int p = q; p < parts; p += 16) s += (double)part[(int64_t)p * D + d];
+    for (int p = q; p < parts; p += 64) s += (double)part[(int64_t)p * D + d];
   }
   red[q][c] = s;
   __syncthreads();
+  if (q < 8) {
+    for (int i = q + 8; i < 64; i += 8) s += red[i][c];
+  }
+  __syncthreads();
+  if (q < 8) red[q][c] = s;
+  __syncthreads();
   if (q == 0 && d < D) {
-    for (int i = 1; i < 16; ++i) s += red[i][c];
+    for (int i = 1; i < 8; ++i) s += red[i][c];
     if (dwt == kF32)
       static_cast<float*>(dw)[d] = (float)s;
     else if (dwt == kBF16)
@@ -277,7 +313,7 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const float* __restrict__ 
   }
 }
 
-// threads per row and 8-value groups per thread: a row within one wave up to 2048 columns (its sums
+// threads per row and 8-value groups per thread: a row within one wave up to 1024 columns (its sums
 // need no barrier), a work-group beyond
 #define PCST_NORM_SHAPES(D, CALL)      \
   do {                                 \
@@ -285,13 +321,13 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const float* __restrict__ 
     else if ((D) <= 256) CALL(32, 1);  \
     else if ((D) <= 512) CALL(64, 1);  \
     else if ((D) <= 1024) CALL(64, 2); \
-    else if ((D) <= 2048) CALL(64, 4); \
+    else if ((D) <= 2048) CALL(256, 1); \
     else if ((D) <= 4096) CALL(256, 2); \
-    else if ((D) <= 8192) CALL(256, 4); \
+    else if ((D) <= 8192) CALL(512, 2); \
     else CALL(512, 4);                 \
   } while (0)
 
-int norm_rpb(int64_t D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 2048 ? 4 : 1; }
+int norm_rpb(int64_t D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 1024 ? 4 : 1; }
 
 template <class T, int QUANT, bool NORM>
 void launch_fwd(const NormArgs& a, hipStream_t s) {
@@ -314,7 +350,7 @@ void launch_bwd(const NormBwdArgs& a, unsigned grid, hipStream_t s) {
 bool is_float(int t) { return t == kF32 || t == kBF16 || t == kF16; }
 
 int64_t norm_parts(int64_t M, int64_t D) {
-  return std::min<int64_t>(cdiv(M, norm_rpb(D)), kNormMaxParts);
+  return std::min<int64_t>(cdiv(M, norm_rpb(D)), D <= kNormNarrow ? kNormPartsNarrow : kNormParts);
 }
 
 int check_dims(const char* who, int64_t M, int64_t D, int dt, int wdt) {
@@ -399,7 +435,7 @@ extern "C" int pcst_rms_norm_bwd(const void* s, int dtype, int64_t M, int64_t D,
     else launch_bwd<_Float16>(a, (unsigned)parts, st);
   }
   if (dw)
-    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)cdiv(D, 16)), dim3(256), 0, st,
+    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)cdiv(D, 16)), dim3(1024), 0, st,
                        static_cast<const float*>(workspace), (int)parts, (int)D, dw, weight_dtype);
   PCST_LAUNCH_CHECK("rms_norm_bwd");
   return PCST_OK;

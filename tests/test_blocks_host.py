@@ -47,7 +47,8 @@ def test_norm_null_pointers_and_no_rows():
     assert rc("pcst_quant_rows", one, 1, 4, 8, one, None, None) == EINVAL
     assert rc("pcst_rms_norm_bwd", one, 1, 4, 8, one, 1, one, one, None, one, one, None, None) == EINVAL  # dw: workspace
     assert rc("pcst_rms_norm", None, None, 1, 0, 8, None, 1, 1e-6, None, None, None, None) == 0  # nothing to do
-    assert size("pcst_rms_norm_bwd_workspace_size", 100000, 256) == (0, 512 * 256 * 4)
+    assert size("pcst_rms_norm_bwd_workspace_size", 100000, 256) == (0, 2048 * 256 * 4)
+    assert size("pcst_rms_norm_bwd_workspace_size", 100000, 4096) == (0, 512 * 4096 * 4)
 
 
 @pytest.mark.parametrize("kw,want", [
