@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(ClipTable t, int64_t ch
 // thread with kFlight loads in flight), which take chunk after chunk and leave one partial each.
 constexpr int kClipGroups = 1024;
 int64_t clip_chunk(int64_t total) {
-  return std::max<int64_t>(2048, std::min<int64_t>(65536, cdiv(cdiv(total, kClipGroups), 2048) * 2048));
+  return std::max<int64_t>(2048, std::min<int64_t>(16384, cdiv(cdiv(total, kClipGroups), 2048) * 2048));
 }
 
 int64_t clip_total(const int64_t* n, int count) {
