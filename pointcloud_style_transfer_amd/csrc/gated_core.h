@@ -40,7 +40,7 @@ typedef __amdgpu_buffer_rsrc_t rsrc_t;
 #define PCST_LDS __attribute__((address_space(3)))
 
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
-enum { EPI_FWD = 0, EPI_BWD = 1, EPI_OUT = 2 };
+enum { EPI_FWD = 0, EPI_BWD = 1, EPI_OUT = 2, EPI_RAW = 3 };  // RAW: g and u of a k split, fp32
 
 constexpr int kRowB = 128;  // bytes of k per stage
 
@@ -258,7 +258,7 @@ __device__ __forceinline__ void load_bias(const void* b, int f32, int64_t f, int
 
 // E: operand type, O: output type, NMN / MMN: the column / row operand's row index is contiguous
 template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, int BM, int BNH, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TNH = BNH / WN / 16;
   constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
   constexpr bool GATED = EPI != EPI_OUT;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
   // The same at the start of a tile, whose stage was loaded before the previous tile's stores: these stay
   // in flight.  kStores of them follow the loads where that tile was a whole one (`stores`); the counter
   // falls in order, so at kStores left, the loads are done.
-  constexpr int kStores = EPI == EPI_FWD ? TM * 4 : TM * TNH * 2;
+  constexpr int kStores = EPI == EPI_FWD ? TM * 4 : EPI == EPI_RAW ? TM * 8 : TM * TNH * 2;
   auto first = [&](bool stores) {
     if (stores && LOOP && EPI != EPI_BWD)
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStores) : "memory");
@@ -458,7 +458,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs g) {
 
   // ---- epilogue
   const int l = lane & 15, q = lane >> 4;
-  if constexpr (GATED) {
+  if constexpr (EPI == EPI_RAW) {
+    const int f = n0 + (wn * 16 + l) * TNH, n = g.N - f;
+    float* out = static_cast<float*>(g.out[0]) + cur.split * g.o_split;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t m = m0 + wm * 16 * TM + 16 * i + 4 * q + r;
+        if (m >= g.M || n <= 0) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[TNH];
+#pragma unroll
+          for (int t = 0; t < TNH; ++t) v[t] = acc[h][t][i][r];
+          store_n<float, TNH>(out + (h * g.M + m) * g.ldo + f, n, v);
+        }
+      }
+  } else if constexpr (GATED) {
     // lane: row 4 q + r of each row tile, TNH consecutive features
     const int f = n0 + (wn * 16 + l) * TNH, n = g.N - f;
     float bg[TNH], bu[TNH], sg[TNH], su[TNH], cg[TNH], cu[TNH];
@@ -649,6 +666,7 @@ struct FwdCall {
   const void *bg, *bu;
   int bias_f32, act, out_type;
   const float *xs, *gs, *us;
+  float* part;  // partial sums of split products
   void* h;
 };
 struct BwdCall {
@@ -656,33 +674,75 @@ struct BwdCall {
   const void* dh;
   void* dgu;       // [M, 2 * fpad]
   int64_t fpad;
-  float *bpart, *wpart;
+  float* bpart;
   void *dx, *dwg, *dwu, *dbg, *dbu;
   int wgrad_f32, bgrad_f32;
 };
 
-constexpr int kBigTiles = 200;  // launches of at least this many large tiles take them
+// ---- which tiles, and over how many splits of k
+// Tiles of 256 x 2*128, 128 x 2*64 and 64 x 2*32; 1, 2 and 4 work-groups of them run on a CU.  The time of a
+// launch is estimated as rounds of work-groups x (stages x a stage's time + a tile's start and end), both
+// measured with the device full (us, 16-bit: 8192 x 4096 x 8192; start and end: 60000 x 512 with k = 64 .. 512);
+// a round that leaves CUs with fewer work-groups is faster by that, down to the latency of a load.  Splitting
+// k costs a launch and the partial sums' way through memory.
+struct Tiling {
+  int bm, bnh, wm, wn, per_cu;
+  double stage[3], ends;  // stage: 16-bit, float, e4m3
+};
+constexpr Tiling kTilings[3] = {{256, 128, 4, 2, 1, {1.8, 7.8, 2.0}, 6.0},
+                                {128, 64, 2, 2, 2, {0.98, 3.9, 1.1}, 3.7},
+                                {64, 32, 2, 2, 4, {0.75, 2.05, 0.9}, 2.0}};
+constexpr double kStageMin = 0.5, kSplitUs = 5.0, kBytesPerUs = 4e6;
 
-inline bool take_big(int64_t M, int64_t N, int nw, int64_t kbytes) { return kbytes >= 128 && cdiv(M, 256) * cdiv(N, nw) >= kBigTiles; }
-
-struct WgradPlan {
-  bool big;
-  int splits;
+struct Plan {
+  int tiling, splits;
   int64_t kps;
 };
-// dW's tiles are few and its k is long: split k until about 512 work-groups run, at least 8 stages each
-inline WgradPlan wgrad_plan(int64_t M, int64_t D, int64_t F, int es) {
-  WgradPlan p;
-  p.big = 2 * cdiv(F, 256) * cdiv(D, 256) >= kBigTiles;
-  const int64_t tiles = p.big ? 2 * cdiv(F, 256) * cdiv(D, 256) : 2 * cdiv(F, 128) * cdiv(D, 128);
-  const int64_t bke = kRowB / es;
-  int64_t s = std::max<int64_t>(1, 512 / tiles);
-  s = std::max<int64_t>(1, std::min<int64_t>(s, cdiv(M, 8 * bke)));
-  p.kps = cdiv(cdiv(M, s), bke) * bke;
-  p.splits = (int)std::max<int64_t>(1, cdiv(M, p.kps));
-  return p;
+
+// rows x cols outputs of `groups` products with `segs` sums of K; wide: a tile is 2 * bnh columns (else the
+// two blocks are Wg's and Wu's); outputs: fp32 values of one partial
+inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bool wide, int es, int64_t outputs) {
+  Plan best{0, 1, K};
+  double least = 1e300;
+  const int64_t bke = kRowB / es, stages = cdiv(K, bke);
+  for (int c = 0; c < 3; ++c) {
+    const Tiling& t = kTilings[c];
+    const double ts = t.stage[es == 4 ? 1 : es == 1 ? 2 : 0];
+    const int64_t tiles = cdiv(rows, t.bm) * cdiv(cols, wide ? 2 * t.bnh : t.bnh) * groups;
+    for (int64_t s = 1; s <= 64 && s <= stages; s *= 2) {
+      if (s > 1 && (c == 0 || tiles * (s / 2) >= 256 * t.per_cu)) break;  // the device is full without
+      const int64_t per = cdiv(stages, s), n = tiles * cdiv(stages, per), slots = 256 * t.per_cu;
+      const double part = std::max(std::min(kStageMin, ts), ts * (double)cdiv(n % slots, 256) / t.per_cu);
+      const double us = (double)(n / slots) * ((double)(per * segs) * ts + t.ends) +
+                        (n % slots ? (double)(per * segs) * part + t.ends : 0.0) +
+                        (s > 1 ? kSplitUs + 8.0 * (double)outputs * (double)s / kBytesPerUs : 0.0);
+      if (us < least) {
+        least = us;
+        best = Plan{c, (int)cdiv(stages, per), s > 1 ? per * bke : K};
+      }
+    }
+  }
+  return best;
 }
-inline int64_t bias_parts(int64_t M, int64_t F, int64_t kbytes) { return take_big(M, F, 128, kbytes) ? cdiv(M, 256) * 4 : cdiv(M, 128) * 2; }
+inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
+inline Plan plan_dx(int64_t M, int64_t D, int64_t F, int es) { return plan(M, D, F, 2, 1, true, es, M * D); }
+inline Plan plan_dw(int64_t M, int64_t D, int64_t F, int es) { return plan(F, D, M, 1, 2, true, es, 2 * F * D); }
+
+// floats of partial sums that a call needs, one product at a time
+inline int64_t part_floats(int64_t M, int64_t D, int64_t F, int es, bool bwd) {
+  auto need = [](const Plan& p, int64_t outputs) { return p.splits > 1 ? p.splits * outputs : 0; };
+  int64_t n = need(plan_gated(M, D, F, es), 2 * M * F);
+  if (bwd) {
+    n = std::max(n, need(plan_dx(M, D, F, es), M * D));
+    n = std::max(n, need(plan_dw(M, D, F, es), 2 * F * D));
+  }
+  return n;
+}
+// rows of bias partials: one for each wave's rows of a tile, or for 64 rows where k is split
+constexpr int kFinishRows = 64;
+inline int64_t bias_parts(int64_t M, const Plan& p) {
+  return p.splits > 1 ? cdiv(M, kFinishRows) : cdiv(M, kTilings[p.tiling].bm) * kTilings[p.tiling].wm;
+}
 
 template <class E>
 int fwd(const FwdCall& c, void* stream);
@@ -690,33 +750,124 @@ template <class E>
 int bwd(const BwdCall& c, void* stream);
 
 #ifdef PCST_GATED_IMPL
-template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, bool BIG>
-int launch(GemmArgs& g, hipStream_t s) {
-  constexpr int BM = BIG ? 256 : 128, BNH = BIG ? 128 : 64, WM = BIG ? 4 : 2, WN = 2;
-  constexpr int NT = EPI == EPI_OUT ? 2 * BNH : BNH;
-  const int64_t tm = cdiv(g.M, BM), tn = cdiv(g.N, NT), n = tm * tn * g.groups * g.splits;
+template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, int C>
+int launch_tiling(GemmArgs& g, hipStream_t s) {
+  constexpr Tiling t = kTilings[C];
+  const int64_t tm = cdiv(g.M, t.bm), tn = cdiv(g.N, EPI == EPI_OUT ? 2 * t.bnh : t.bnh), n = tm * tn * g.groups * g.splits;
   PCST_CHECK_ARG(n < (1ll << 30), "gated_linear: too many tiles");
   g.tiles_m = (int)tm;
   g.tiles_n = (int)tn;
   g.ntiles = (int)n;
   g.per_xcd = (int)cdiv(n, 8);
-  // small tiles: as many work-groups as run at a time (two on each of 256 CUs)
-  const unsigned grid = (unsigned)(BIG ? g.per_xcd * 8 : std::min<int64_t>(g.per_xcd * 8, 512));
-  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, ACT, BM, BNH, WM, WN>), dim3(grid),
-                     dim3(64 * WM * WN), 0, s, g);
+  // the smaller tiles: as many work-groups as run at a time
+  const unsigned grid = (unsigned)(C == 0 ? g.per_xcd * 8 : std::min<int64_t>(g.per_xcd * 8, 256 * t.per_cu));
+  hipLaunchKernelGGL((gemm_kernel<E, O, NMN, MMN, EPI, ACT, t.bm, t.bnh, t.wm, t.wn>), dim3(grid),
+                     dim3(64 * t.wm * t.wn), 0, s, g);
+  PCST_LAUNCH_CHECK("gated_linear");
+  return PCST_OK;
+}
+template <class E, class O, bool NMN, bool MMN, int EPI, int ACT>
+int launch(GemmArgs& g, int tiling, hipStream_t s) {
+  if (tiling == 0 && EPI != EPI_RAW) return launch_tiling<E, O, NMN, MMN, EPI, ACT, EPI == EPI_RAW ? 1 : 0>(g, s);
+  return tiling == 1 ? launch_tiling<E, O, NMN, MMN, EPI, ACT, 1>(g, s) : launch_tiling<E, O, NMN, MMN, EPI, ACT, 2>(g, s);
+}
+template <class E, class O, int EPI>
+int launch_act(GemmArgs& g, int tiling, int act, hipStream_t s) {
+  return act == ACT_SILU   ? launch<E, O, false, false, EPI, ACT_SILU>(g, tiling, s)
+         : act == ACT_GELU ? launch<E, O, false, false, EPI, ACT_GELU>(g, tiling, s)
+                           : launch<E, O, false, false, EPI, ACT_RELU>(g, tiling, s);
+}
+
+// ---- the gated epilogues behind a split k: the splits added in order, then as above.  A work-group takes 64
+// features of kFinishRows rows.
+struct FinishArgs {
+  const float* part;  // [splits, 2, M, F]
+  int splits;
+  int64_t M;
+  int F;
+  const void *bg, *bu;
+  int bias_f32;
+  const float *xs, *gs, *us;
+  const void* dh;
+  void* out;
+  int64_t ldo, fpad;
+  float* bpart;
+};
+template <class E, class O, int EPI, int ACT>
+__global__ __launch_bounds__(256) void finish_kernel(FinishArgs a) {
+  constexpr bool FAST = elem_size<E>() < 4;
+  __shared__ float red[2][4][64];
+  const int c = threadIdx.x & 63, w = threadIdx.x >> 6, f = blockIdx.x * 64 + c;
+  const int64_t m0 = (int64_t)blockIdx.y * kFinishRows, n = a.M * a.F;
+  const bool in = f < a.F;
+  float bg[1] = {0.f}, bu[1] = {0.f}, cg = 0.0f, cu = 0.0f;
+  if (in) {
+    load_bias<O, 1>(a.bg, a.bias_f32, f, 1, bg);
+    load_bias<O, 1>(a.bu, a.bias_f32, f, 1, bu);
+  }
+  for (int64_t m = m0 + w; m < m0 + kFinishRows && m < a.M; m += 4) {
+    float g = 0.0f, u = 0.0f;
+    if (in) {
+      const float* p = a.part + m * a.F + f;
+#pragma unroll 4
+      for (int k = 0; k < a.splits; ++k) {
+        g += p[2 * k * n];
+        u += p[(2 * k + 1) * n];
+      }
+      if (elem_size<E>() == 1) {
+        g *= a.xs[m] * a.gs[f];
+        u *= a.xs[m] * a.us[f];
+      }
+      g += bg[0];
+      u += bu[0];
+    }
+    if (EPI == EPI_FWD) {
+      if (in) static_cast<O*>(a.out)[m * a.ldo + f] = (O)(act_value<FAST, ACT>(g) * u);
+    } else {  // (f < fpad: a multiple of 64)
+      float v, og = 0.0f, ou = 0.0f;
+      const float da = act_grad<FAST, ACT>(g, v);
+      if (in) {
+        const float d = (float)static_cast<const O*>(a.dh)[m * a.F + f];
+        og = d * u * da;
+        ou = d * v;
+        cg += og;
+        cu += ou;
+      }
+      static_cast<O*>(a.out)[m * a.ldo + f] = (O)og;
+      static_cast<O*>(a.out)[m * a.ldo + a.fpad + f] = (O)ou;
+    }
+  }
+  if (EPI == EPI_BWD && a.bpart) {
+    red[0][w][c] = cg;
+    red[1][w][c] = cu;
+    __syncthreads();
+    if (w < 2 && in)
+      a.bpart[((int64_t)blockIdx.y * 2 + w) * a.F + f] = red[w][0][c] + red[w][1][c] + red[w][2][c] + red[w][3][c];
+  }
+}
+template <class E, class O, int EPI>
+int launch_finish(const FinishArgs& a, int act, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.F, 64), (unsigned)cdiv(a.M, kFinishRows));
+  if (act == ACT_SILU) hipLaunchKernelGGL((finish_kernel<E, O, EPI, ACT_SILU>), grid, dim3(256), 0, s, a);
+  else if (act == ACT_GELU) hipLaunchKernelGGL((finish_kernel<E, O, EPI, ACT_GELU>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((finish_kernel<E, O, EPI, ACT_RELU>), grid, dim3(256), 0, s, a);
   PCST_LAUNCH_CHECK("gated_linear");
   return PCST_OK;
 }
 
-// the forward and the recomputing backward, by activation and tile
+// the forward (EPI_FWD, into out) or the recomputing backward (EPI_BWD, into [dg | du])
 template <class E, class O, int EPI>
-int launch_gated(GemmArgs& g, hipStream_t s, int act) {
-  const bool big = take_big(g.M, g.N, 128, g.K * elem_size<E>());
-  if (act == ACT_SILU)
-    return big ? launch<E, O, false, false, EPI, ACT_SILU, true>(g, s) : launch<E, O, false, false, EPI, ACT_SILU, false>(g, s);
-  if (act == ACT_GELU)
-    return big ? launch<E, O, false, false, EPI, ACT_GELU, true>(g, s) : launch<E, O, false, false, EPI, ACT_GELU, false>(g, s);
-  return big ? launch<E, O, false, false, EPI, ACT_RELU, true>(g, s) : launch<E, O, false, false, EPI, ACT_RELU, false>(g, s);
+int run_gated(GemmArgs& g, const Plan& p, int act, float* part, hipStream_t s) {
+  if (p.splits == 1) return launch_act<E, O, EPI>(g, p.tiling, act, s);
+  const FinishArgs a{part,  p.splits, g.M, g.N, g.bg, g.bu, g.bias_f32, g.xs, g.gs, g.us, g.dh, g.out[0], g.ldo, g.fpad,
+                     g.bpart};
+  g.splits = p.splits;
+  g.kps = p.kps;
+  g.out[0] = part;
+  g.ldo = g.N;
+  g.o_split = 2 * g.M * g.N;
+  if (int rc = launch<E, float, false, false, EPI_RAW, 0>(g, p.tiling, s)) return rc;
+  return launch_finish<E, O, EPI>(a, act, s);
 }
 
 inline GemmArgs fwd_args(const FwdCall& c) {
@@ -758,7 +909,7 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
     return c.act == ACT_SILU   ? launch_rows<E, O, ACT_SILU>(g, s)
            : c.act == ACT_GELU ? launch_rows<E, O, ACT_GELU>(g, s)
                                : launch_rows<E, O, ACT_RELU>(g, s);
-  return launch_gated<E, O, EPI_FWD>(g, s, c.act);
+  return run_gated<E, O, EPI_FWD>(g, plan_gated(c.M, c.D, c.F, elem_size<E>()), c.act, c.part, s);
 }
 
 // dW's partials (one of n values per split and matrix) added in order; blockIdx.y: the matrix
@@ -793,9 +944,22 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ par
   }
 }
 
-template <class E, class O>
-int wgrad_launch(GemmArgs& w, bool big, hipStream_t s) {
-  return big ? launch<E, O, true, true, EPI_OUT, 0, true>(w, s) : launch<E, O, true, true, EPI_OUT, 0, false>(w, s);
+// a plain product (dx, or dWg and dWu as two groups), over splits of k where the plan has them
+template <class E, class O, bool NMN, bool MMN>
+int run_product(GemmArgs& g, const Plan& p, float* part, hipStream_t s) {
+  if (p.splits == 1) return launch<E, O, NMN, MMN, EPI_OUT, 0>(g, p.tiling, s);
+  const int64_t n = g.M * g.N;
+  O *o0 = static_cast<O*>(g.out[0]), *o1 = static_cast<O*>(g.out[1]);
+  g.splits = p.splits;
+  g.kps = p.kps;
+  g.out[0] = part;
+  g.out[1] = part + n;
+  g.o_split = g.groups * n;
+  if (int rc = launch<E, float, NMN, MMN, EPI_OUT, 0>(g, p.tiling, s)) return rc;
+  hipLaunchKernelGGL(combine_kernel<O>, dim3((unsigned)cdiv(n, 256), (unsigned)g.groups), dim3(256), 0, s, part, n,
+                     p.splits, o0, o1);
+  PCST_LAUNCH_CHECK("gated_linear_bwd");
+  return PCST_OK;
 }
 
 template <class E>
@@ -809,11 +973,12 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   g.fpad = c.fpad;
   g.dh = c.dh;
   g.bpart = c.dbg || c.dbu ? c.bpart : nullptr;
-  int rc = launch_gated<E, T, EPI_BWD>(g, s, f.act);
+  const Plan pg = plan_gated(f.M, f.D, f.F, ES);
+  int rc = run_gated<E, T, EPI_BWD>(g, pg, f.act, f.part, s);
   if (rc) return rc;
   if (g.bpart) {
     const dim3 grid((unsigned)cdiv(2 * f.F, 16));
-    const int parts = (int)bias_parts(f.M, f.F, f.D * ES);
+    const int parts = (int)bias_parts(f.M, pg);
     if (c.bgrad_f32)
       hipLaunchKernelGGL(bias_kernel<float>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts,
                          static_cast<float*>(c.dbg), static_cast<float*>(c.dbu));
@@ -836,12 +1001,12 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.splits = d.groups = 1;
     d.out[0] = c.dx;
     d.ldo = f.D;
-    rc = take_big(f.M, f.D, 256, 2 * f.F * ES) ? launch<E, T, true, false, EPI_OUT, 0, true>(d, s)
-                                 : launch<E, T, true, false, EPI_OUT, 0, false>(d, s);
+    const Plan p = plan_dx(f.M, f.D, f.F, ES);
+    rc = run_product<E, T, true, false>(d, p, f.part, s);
     if (rc) return rc;
   }
   if (c.dwg || c.dwu) {
-    const WgradPlan p = wgrad_plan(f.M, f.D, f.F, ES);
+    const Plan p = plan_dw(f.M, f.D, f.F, ES);
     GemmArgs w{};
     w.a[0] = static_cast<const char*>(c.dgu);
     w.b0[0] = static_cast<const char*>(f.x);
@@ -849,9 +1014,8 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     w.ldb = f.ldx;
     w.M = f.F;
     w.N = (int)f.D;
-    w.K = f.M;
-    w.kps = p.kps;
-    w.splits = p.splits;
+    w.K = w.kps = f.M;
+    w.splits = 1;
     w.ldo = f.D;
     void* outs[2] = {c.dwg, c.dwu};
     for (int k = 0; k < 2; ++k)
@@ -859,26 +1023,8 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
         w.a_group[w.groups] = k * c.fpad * ES;
         w.out[w.groups++] = outs[k];
       }
-    if (p.splits == 1) {
-      rc = c.wgrad_f32 ? wgrad_launch<E, float>(w, p.big, s) : wgrad_launch<E, T>(w, p.big, s);
-      if (rc) return rc;
-    } else {
-      const int64_t n = f.F * f.D;
-      void *o0 = w.out[0], *o1 = w.out[1];
-      w.out[0] = c.wpart;
-      w.out[1] = c.wpart + n;
-      w.o_split = w.groups * n;
-      rc = wgrad_launch<E, float>(w, p.big, s);
-      if (rc) return rc;
-      const dim3 grid((unsigned)cdiv(n, 256), (unsigned)w.groups);
-      if (c.wgrad_f32)
-        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, s, c.wpart, n, p.splits,
-                           static_cast<float*>(o0), static_cast<float*>(o1));
-      else
-        hipLaunchKernelGGL(combine_kernel<T>, grid, dim3(256), 0, s, c.wpart, n, p.splits, static_cast<T*>(o0),
-                           static_cast<T*>(o1));
-      PCST_LAUNCH_CHECK("gated_linear_bwd");
-    }
+    rc = c.wgrad_f32 ? run_product<E, float, true, true>(w, p, f.part, s) : run_product<E, T, true, true>(w, p, f.part, s);
+    if (rc) return rc;
   }
   return PCST_OK;
 }

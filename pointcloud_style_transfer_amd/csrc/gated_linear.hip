@@ -35,25 +35,28 @@ struct Layout {
   int64_t pitch;  // bytes of a padded row of D values
   void *x, *wg, *wu;
   void* dgu;
-  float *bpart, *wpart;
+  float *bpart, *part;
   int64_t fpad;
   size_t bytes;
 };
 
-Layout lay(void* ws, int dt, int64_t M, int64_t D, int64_t F, bool bwd) {
+// pad: x, Wg and Wu (or some of them) need copies
+Layout lay(void* ws, int dt, int64_t M, int64_t D, int64_t F, bool pad, bool bwd) {
   Layout l{};
   Carver c(ws);
   const int es = elem(dt);
   l.pitch = cdiv(D * es, 16) * 16;
-  l.x = c.take<char>((size_t)(M * l.pitch));
-  l.wg = c.take<char>((size_t)(F * l.pitch));
-  l.wu = c.take<char>((size_t)(F * l.pitch));
+  if (pad) {
+    l.x = c.take<char>((size_t)(M * l.pitch));
+    l.wg = c.take<char>((size_t)(F * l.pitch));
+    l.wu = c.take<char>((size_t)(F * l.pitch));
+  }
   l.fpad = cdiv(F, 64) * 64;
   if (bwd) {
     l.dgu = c.take<char>((size_t)(M * 2 * l.fpad * es));
-    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, F, D * es) * 2 * F));
-    l.wpart = c.take<float>((size_t)(gated::wgrad_plan(M, D, F, es).splits * 2 * F * D));
+    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, gated::plan_gated(M, D, F, es)) * 2 * F));
   }
+  l.part = c.take<float>((size_t)gated::part_floats(M, D, F, es, bwd));
   l.bytes = c.bytes();
   return l;
 }
@@ -102,7 +105,8 @@ extern "C" int pcst_gated_linear_workspace_size(int dtype, int64_t M, int64_t D,
                                                 size_t* bytes) {
   if (int rc = check("gated_linear_workspace_size", dtype, M, D, F, 0)) return rc;
   PCST_CHECK_ARG(bytes, "gated_linear_workspace_size: null pointer");
-  *bytes = M <= gated::kRowsMax || (aligned && (D * elem(dtype)) % 16 == 0) ? 0 : lay(nullptr, dtype, M, D, F, false).bytes;
+  const bool pad = !aligned || (D * elem(dtype)) % 16 != 0;
+  *bytes = M <= gated::kRowsMax ? 0 : lay(nullptr, dtype, M, D, F, pad, false).bytes;
   return PCST_OK;
 }
 
@@ -123,8 +127,9 @@ extern "C" int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D,
   PCST_CHECK_ARG(x && w_gate && w_up && h, "gated_linear: null pointer");
   const int es = elem(dtype);
   const bool rows = M <= gated::kRowsMax;
-  const bool direct = rows || (ready(x, D, es) && ready(w_gate, D, es) && ready(w_up, D, es));
-  PCST_CHECK_ARG(direct || workspace, "gated_linear: rows off 16-byte boundaries need the workspace");
+  const bool pad = !ready(x, D, es) || !ready(w_gate, D, es) || !ready(w_up, D, es);
+  const Layout l = lay(workspace, dtype, M, D, F, pad, false);
+  PCST_CHECK_ARG(rows || l.bytes == 0 || workspace, "gated_linear: null workspace");
   gated::FwdCall c{};
   c.M = M;
   c.D = D;
@@ -135,7 +140,8 @@ extern "C" int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D,
     c.wu = w_up;
     c.ldx = c.ldw = D * es;
   } else {
-    operands(c, lay(workspace, dtype, M, D, F, false), x, w_gate, w_up, es, as_stream(stream));
+    operands(c, l, x, w_gate, w_up, es, as_stream(stream));
+    c.part = l.part;
   }
   c.bg = b_gate;
   c.bu = b_up;
@@ -157,7 +163,7 @@ extern "C" int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D,
 extern "C" int pcst_gated_linear_bwd_workspace_size(int dtype, int64_t M, int64_t D, int64_t F, size_t* bytes) {
   if (int rc = check("gated_linear_bwd_workspace_size", dtype, M, D, F, 0)) return rc;
   PCST_CHECK_ARG(bytes && dtype != kE4M3, "gated_linear_bwd_workspace_size: bad args");
-  *bytes = lay(nullptr, dtype, M, D, F, true).bytes;
+  *bytes = lay(nullptr, dtype, M, D, F, true, true).bytes;
   return PCST_OK;
 }
 
@@ -172,7 +178,7 @@ extern "C" int pcst_gated_linear_bwd(const void* x, int dtype, int64_t M, int64_
   PCST_CHECK_ARG(M > 0, "gated_linear_bwd: no rows (the gradients of the weights are zero)");
   PCST_CHECK_ARG(x && w_gate && w_up && dh && workspace, "gated_linear_bwd: null pointer");
   const int es = elem(dtype);
-  const Layout l = lay(workspace, dtype, M, D, F, true);
+  const Layout l = lay(workspace, dtype, M, D, F, true, true);
   gated::BwdCall c{};
   c.f.M = M;
   c.f.D = D;
@@ -186,7 +192,7 @@ extern "C" int pcst_gated_linear_bwd(const void* x, int dtype, int64_t M, int64_
   c.dgu = l.dgu;
   c.fpad = l.fpad;
   c.bpart = l.bpart;
-  c.wpart = l.wpart;
+  c.f.part = l.part;
   c.dx = dx;
   c.dwg = dw_gate;
   c.dwu = dw_up;
