@@ -24,6 +24,8 @@
 // the time).  In the forward, W's rows are dealt to the tiles so that a lane's tiles are consecutive
 // features and 16 lanes a whole 128-byte line.
 #pragma once
+#include <type_traits>
+
 #include "ops_types.h"
 
 namespace pcst {
@@ -67,9 +69,8 @@ struct GemmArgs {
   const float *xs, *gs, *us;  // e4m3 scales
 };
 
-__device__ __forceinline__ rsrc_t make_rsrc(const char* p, int64_t bytes) {
-  const int n = bytes <= 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : (int)bytes;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, n, 0x00020000);
+__device__ __forceinline__ rsrc_t make_rsrc(const char* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, bytes > 0 ? bytes : 0, 0x00020000);
 }
 
 template <class E>
@@ -165,8 +166,8 @@ struct Stage {
   static constexpr int ES = elem_size<E>();
   static constexpr int RB = R * ES;          // MN: bytes of one k row
   static constexpr int CPR = RB / 16;
-  static constexpr int IT = R / 8 / NW;      // 1 KiB loads per wave
-  static_assert(R % (8 * NW) == 0, "whole loads per wave");
+  static constexpr int IT = R * kRowB / 1024 / NW;  // 1 KiB loads per wave
+  static_assert(R * kRowB % (1024 * NW) == 0, "whole loads per wave");
   uint32_t off[IT];
   int piece[IT];  // KC: byte offset of the piece in its row (for the end of k)
 
@@ -188,7 +189,7 @@ struct Stage {
   }
   // base: the tile's first byte at this stage's first k; bytes: up to the end of what may be read;
   // kleft: bytes of k left (KC)
-  __device__ __forceinline__ void load(PCST_LDS char* img, const char* base, int64_t bytes, int kleft, int wave) const {
+  __device__ __forceinline__ void load(PCST_LDS char* img, const char* base, int bytes, int kleft, int wave) const {
     const rsrc_t r = make_rsrc(base, bytes);
 #pragma unroll
     for (int j = 0; j < IT; ++j) {
@@ -256,13 +257,65 @@ __device__ __forceinline__ void load_bias(const void* b, int f32, int64_t f, int
   }
 }
 
+// The gated epilogue of one wave: acc[0] (g) and acc[1] (u) of TM tiles of 16 rows, the lane's rows m + 16 i
+// + 0..3, and TNH consecutive features from f on -> h, or [dg | du] and their column sums (before rounding)
+template <class E, class O, int EPI, int ACT, int TM, int TNH>
+__device__ __forceinline__ void gated_rows(const GemmArgs& g, const f32x4 (&acc)[2][TNH][TM], int64_t m0, int f,
+                                           const float (&bg)[TNH], const float (&bu)[TNH], const float (&sg)[TNH],
+                                           const float (&su)[TNH], float (&cg)[TNH], float (&cu)[TNH]) {
+  constexpr int ES = elem_size<E>();
+  constexpr bool FAST = ES < 4;
+  const int n = g.N - f;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t m = m0 + 16 * i + r;
+      if (m >= g.M) continue;
+      float gv[TNH], uv[TNH];
+      const float xs = ES == 1 ? g.xs[m] : 1.0f;
+#pragma unroll
+      for (int t = 0; t < TNH; ++t) {
+        gv[t] = acc[0][t][i][r];
+        uv[t] = acc[1][t][i][r];
+        if (ES == 1) {
+          gv[t] *= xs * sg[t];
+          uv[t] *= xs * su[t];
+        }
+        gv[t] += bg[t];
+        uv[t] += bu[t];
+      }
+      if (EPI == EPI_FWD) {
+        float o[TNH];
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) o[t] = act_value<FAST, ACT>(gv[t]) * uv[t];
+        if (n > 0) store_n<O, TNH>(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
+      } else if (f < g.fpad) {
+        float d[TNH], og[TNH], ou[TNH];
+        load_bias<O, TNH>(g.dh, 0, m * g.N + f, n, d);
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) {
+          float v;
+          const float da = act_grad<FAST, ACT>(gv[t], v);
+          og[t] = t < n ? d[t] * uv[t] * da : 0.0f;  // the padding up to fpad is zero
+          ou[t] = t < n ? d[t] * v : 0.0f;
+          cg[t] += og[t];
+          cu[t] += ou[t];
+        }
+        O* o = static_cast<O*>(g.out[0]) + m * g.ldo + f;
+        store_n<O, TNH>(o, TNH, og);
+        store_n<O, TNH>(o + g.fpad, TNH, ou);
+      }
+    }
+  }
+}
+
 // E: operand type, O: output type, NMN / MMN: the column / row operand's row index is contiguous
 template <class E, class O, bool NMN, bool MMN, int EPI, int ACT, int BM, int BNH, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(GemmArgs g) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TNH = BNH / WN / 16;
   constexpr int ES = elem_size<E>(), BKE = kRowB / ES;
   constexpr bool GATED = EPI != EPI_OUT;
-  constexpr bool FAST = ES < 4;
   constexpr int NSEG = NMN && !MMN ? 2 : 1;  // k segments: dx sums over Wg, then over Wu
   constexpr bool LOOP = WM * WN == 4;  // several tiles a work-group
   static_assert(!GATED || !NMN, "the forward reads W with k contiguous");
@@ -294,7 +347,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
     int n0, tm, group, split, nk, total;
     int64_t klen;  // of a segment
     const char *pa[NSEG], *pb0[NSEG], *pb1[NSEG];  // per k segment, at its first k
-    int64_t ra, rb0, rb1;                 // bytes that may be read from there
+    int ra, rb0, rb1;  // KC: bytes that may be read from there; MN: bytes of a row in front of the tile
   };
   auto decode = [&](int L, Tile& c) -> bool {
     const int idx = L >> 3;
@@ -318,9 +371,10 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
     const int64_t rows = g.M - c.m0 < BM ? g.M - c.m0 : BM;
     const int64_t cols = g.N - c.n0 < BNH ? g.N - c.n0 : BNH;
     const int64_t cols1 = GATED ? cols : g.N - c.n0 - BNH < BNH ? g.N - c.n0 - BNH : BNH;
-    c.ra = MMN ? c.klen * g.lda - c.m0 * ES : rows * g.lda - kb * ES;
-    c.rb0 = NMN ? c.klen * g.ldb - (int64_t)c.n0 * ES : cols * g.ldb - kb * ES;
-    c.rb1 = cols1 * g.ldb - kb * ES;  // (NMN: not used)
+    // (a tile's rows, and a stage's, are less than 2^31 bytes: the C entry's bounds)
+    c.ra = MMN ? (int)(c.m0 * ES) : (int)(rows * g.lda - kb * ES);
+    c.rb0 = NMN ? c.n0 * ES : (int)(cols * g.ldb - kb * ES);
+    c.rb1 = (int)((cols1 > 0 ? cols1 : 0) * g.ldb - kb * ES);  // (NMN: not used)
 #pragma unroll
     for (int q = 0; q < NSEG; ++q) {
       c.pa[q] = g.a[q] + g.a_group[c.group] + (MMN ? kb * g.lda + c.m0 * ES : c.m0 * g.lda + kb * ES);
@@ -335,30 +389,38 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
     const int seg = NSEG > 1 && it >= c.nk ? 1 : 0;
     const int k = it - (seg ? c.nk : 0);
     const int64_t oa = k * step_a, ob = k * step_b;
-    const int64_t left = c.klen * ES - (int64_t)k * kRowB;
-    const int kl = left > kRowB ? kRowB : (int)left;
-    sa.load(ia, c.pa[seg] + oa, c.ra - oa, kl, wave);
-    sb.load(ib, c.pb0[seg] + ob, c.rb0 - ob, kl, wave);
-    if (!NMN) sb.load(ib + BNH * kRowB, c.pb1[seg] + ob, c.rb1 - ob, kl, wave);
+    const int64_t left = c.klen - (int64_t)k * BKE;  // elements of k
+    const int kn = left > BKE ? BKE : (int)left, kl = kn * ES;
+    sa.load(ia, c.pa[seg] + oa, MMN ? kn * (int)g.lda - c.ra : c.ra - k * kRowB, kl, wave);
+    sb.load(ib, c.pb0[seg] + ob, NMN ? kn * (int)g.ldb - c.rb0 : c.rb0 - k * kRowB, kl, wave);
+    if (!NMN) sb.load(ib + BNH * kRowB, c.pb1[seg] + ob, c.rb1 - k * kRowB, kl, wave);
   };
 
   f32x4 acc[2][TNH][TM];
   auto compute = [&](const PCST_LDS char* ia, const PCST_LDS char* ib, auto&& prefetch) {
     if constexpr (ES == 1) {
-      i32x4 a[2][TM];
+      // a stage is one product deep; the fragments of two column tiles are read ahead of their products
+      i32x4 a[2][TM], b[3][2];
+      auto read_b = [&](int n) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks) b[n % 3][ks] = fb[0].read(ib + n / TNH * BNH * kRowB, n % TNH, ks);
+      };
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[ks][i] = fa.read(ia, i, ks);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) a[ks][i] = fa.read(ia, i, ks);
+      read_b(0);
+      read_b(1);
+      __builtin_amdgcn_sched_barrier(0);
       prefetch();
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int n = 0; n < 2 * TNH; ++n) {
+        if (n + 2 < 2 * TNH) read_b(n + 2);
 #pragma unroll
-        for (int j = 0; j < TNH; ++j) {
-          const i32x4 b0 = fb[0].read(ib + h * BNH * kRowB, j, 0), b1 = fb[0].read(ib + h * BNH * kRowB, j, 1);
-#pragma unroll
-          for (int i = 0; i < TM; ++i) acc[h][j][i] = mma32_e4m3(a[0][i], a[1][i], b0, b1, acc[h][j][i]);
-        }
+        for (int i = 0; i < TM; ++i)
+          acc[n / TNH][n % TNH][i] = mma32_e4m3(a[0][i], a[1][i], b[n % 3][0], b[n % 3][1], acc[n / TNH][n % TNH][i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     } else {
       // four groups (k step, column block) of TM * TNH products; a group's products run while the next
       // one's fragments are read
@@ -382,9 +444,16 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
       read_b(0, 0);
       read_b(0, 1);
       __builtin_amdgcn_sched_barrier(0);
-      prefetch();  // the other stage's loads, behind this one's first reads
+      prefetch();  // the other stage's loads, behind this one's first reads and between the products
       mma(0, 0);
       read_a(1);
+#pragma unroll
+      for (int n = 0; n < TM * TNH; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // an MFMA,
+        __builtin_amdgcn_sched_group_barrier(0x006, 6, 0);   // what prepares a load,
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);   // a load,
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // a fragment
+      }
       __builtin_amdgcn_sched_barrier(0);
       read_b(1, 0);
       mma(0, 1);
@@ -487,49 +556,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
     }
 #pragma unroll
     for (int t = 0; t < TNH; ++t) cg[t] = cu[t] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int64_t mi = m0 + wm * 16 * TM + 16 * i + 4 * q;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t m = mi + r;
-        if (m >= g.M) continue;
-        float gv[TNH], uv[TNH];
-        const float xs = ES == 1 ? g.xs[m] : 1.0f;
-#pragma unroll
-        for (int t = 0; t < TNH; ++t) {
-          gv[t] = acc[0][t][i][r];
-          uv[t] = acc[1][t][i][r];
-          if (ES == 1) {
-            gv[t] *= xs * sg[t];
-            uv[t] *= xs * su[t];
-          }
-          gv[t] += bg[t];
-          uv[t] += bu[t];
-        }
-        if (EPI == EPI_FWD) {
-          float o[TNH];
-#pragma unroll
-          for (int t = 0; t < TNH; ++t) o[t] = act_value<FAST, ACT>(gv[t]) * uv[t];
-          if (n > 0) store_n<O, TNH>(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
-        } else if (f < g.fpad) {
-          float d[TNH], og[TNH], ou[TNH];
-          load_bias<O, TNH>(g.dh, 0, m * g.N + f, n, d);
-#pragma unroll
-          for (int t = 0; t < TNH; ++t) {
-            float v;
-            const float da = act_grad<FAST, ACT>(gv[t], v);
-            og[t] = t < n ? d[t] * uv[t] * da : 0.0f;  // the padding up to fpad is zero
-            ou[t] = t < n ? d[t] * v : 0.0f;
-            cg[t] += og[t];
-            cu[t] += ou[t];
-          }
-          O* o = static_cast<O*>(g.out[0]) + m * g.ldo + f;
-          store_n<O, TNH>(o, TNH, og);
-          store_n<O, TNH>(o + g.fpad, TNH, ou);
-        }
-      }
-    }
+    gated_rows<E, O, EPI, ACT>(g, acc, m0 + wm * 16 * TM + 4 * q, f, bg, bu, sg, su, cg, cu);
     if (EPI == EPI_BWD && g.bpart) {  // column sums of the wave's rows, before rounding
       float* bp = g.bpart + ((int64_t)tm * WM + wm) * 2 * g.N + f;
 #pragma unroll
@@ -659,6 +686,158 @@ __global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
   }
 }
 
+// ---- narrow rows (K of at most 512 bytes, many rows): a work-group keeps 128 features of both matrices in
+// LDS for its whole life, and each of its waves takes tiles of 64 rows by itself, straight from memory into
+// registers: no barrier after the start, so that one wave's epilogue runs beside the other's products, and
+// x is read once for every 128 features instead of W once for every 256 rows.  The next tile's rows are
+// loaded as this one's are used for the last time.
+constexpr int kNarrowF = 128, kNarrowBytes = 512;
+// rows of a wave's tile: what the registers hold of x beside the sums
+__host__ __device__ constexpr int narrow_rows_of(int64_t kbytes) { return kbytes <= 256 ? 64 : 48; }
+
+// The forward's epilogue of narrow_kernel (whose sums hold the biases): 2 features of a 16-bit output,
+// addressed with 32 bits from the tile's first row (vo: the lane's offset; a row's is scalar).  FULL: all rows,
+// both features and 4-byte stores; else each value by itself, behind its limits.
+template <class O, int ACT, bool FULL, int TM>
+__device__ __forceinline__ void narrow_rows(const f32x4 (&acc)[2][2][TM], rsrc_t out, int vo, int pitch, int rows, int n) {
+  typedef typename Vec<O, 2>::V V2;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * i + r;  // and 4 q, which vo and rows hold
+      V2 o;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) o[t] = (O)(act_value<true, ACT>(acc[0][t][i][r]) * acc[1][t][i][r]);
+      if (FULL) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, o), out, vo, row * pitch, 0);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (row < rows && t < n)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (O)o[t]), out, vo + 2 * t, row * pitch, 0);
+      }
+    }
+}
+
+template <class E, class O, int ACT, int KS>
+__global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
+  constexpr int ES = elem_size<E>(), kNarrowRows = narrow_rows_of(KS * 64), TM = kNarrowRows / 16, TNH = 2;
+  constexpr int IM = KS / 2, SG = kNarrowF / 32;
+  __shared__ __attribute__((aligned(1024))) char lds_w[IM * 2 * kNarrowF * kRowB];
+  __shared__ float lds_b[2][kNarrowF];                                   // biases
+  // tiles_n blocks of features x tiles_m groups of rows; an XCD's work-groups share row groups
+  const int L = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
+  if (L >= g.ntiles) return;
+  const int rg = L / g.tiles_n, n0 = (L - rg * g.tiles_n) * kNarrowF;
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kb = (int)g.K * ES;
+  PCST_LDS char* w = (PCST_LDS char*)lds_w;
+  {
+    Stage<E, false, kNarrowF, TNH, 8> sw;
+    sw.init(wave, lane, g.ldb);
+    const int rows = g.N - n0 < kNarrowF ? g.N - n0 : kNarrowF;
+#pragma unroll
+    for (int im = 0; im < IM; ++im)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        sw.load(w + (im * 2 + h) * kNarrowF * kRowB, (h ? g.b1[0] : g.b0[0]) + (int64_t)n0 * g.ldb + im * kRowB,
+                (int)(rows * g.ldb) - im * kRowB, kb - im * kRowB, wave);
+    if (tid < kNarrowF) {
+      float v[1];
+      load_bias<O, 1>(g.bg, g.bias_f32, n0 + tid, g.N - n0 - tid, v);
+      lds_b[0][tid] = v[0];
+      load_bias<O, 1>(g.bu, g.bias_f32, n0 + tid, g.N - n0 - tid, v);
+      lds_b[1][tid] = v[0];
+    }
+  }
+  Frag<E, false, kNarrowF, TNH> fb;
+  fb.init(0, lane);
+
+  // of the two waves of a SIMD, one goes first through its products: they come apart, and one's epilogue
+  // runs beside the other's products
+  const bool ahead = wave < 4;
+  i32x4 x[TM][KS];
+  // 4-byte accesses of pairs of features: all 128 there, and rows on 4-byte boundaries
+  const bool whole = n0 + kNarrowF <= g.N && (g.N & 1) == 0 && ((uintptr_t)g.out[0] & 3) == 0;
+  const int step = g.tiles_m * 8, tiles = (int)((g.M + kNarrowRows - 1) / kNarrowRows);
+  int tile = rg * 8 + wave;
+  auto tile_rsrc = [&](int t) {
+    const int64_t m0 = (int64_t)t * kNarrowRows, rows = g.M - m0 < kNarrowRows ? g.M - m0 : kNarrowRows;
+    return make_rsrc(g.a[0] + m0 * g.lda, t < tiles ? (int)(rows * g.lda) : 0);  // past the last tile: fetches nothing
+  };
+  auto load_x = [&](rsrc_t r, int i, int ks) {
+    const int o = ks * 64 + q * 16 < kb ? (int)((16 * i + l) * g.lda) + ks * 64 + q * 16 : (int)0x80000000;
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+  };
+  {
+    const rsrc_t r = tile_rsrc(tile);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) x[i][ks] = load_x(r, i, ks);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+
+  for (; tile < tiles; tile += step) {
+    const int64_t mt = (int64_t)tile * kNarrowRows;
+    const rsrc_t ro = make_rsrc(static_cast<char*>(g.out[0]) + mt * g.ldo * 2, 0x7fffffff);
+    const bool full = whole && mt + kNarrowRows <= g.M;
+    const rsrc_t rn = tile_rsrc(tile + step);
+    auto group = [&](int sgi, auto last) {
+      // the sums start at the biases
+      const int c = sgi * 32 + l * TNH;
+      f32x4 acc[2][TNH][TM], c0[2][TNH];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) {
+          const float v = lds_b[h][c + t];
+          c0[h][t] = f32x4{v, v, v, v};
+        }
+      const PCST_LDS char* ws = w + sgi * 32 * kRowB;
+      i32x4 b[2][2][TNH];
+      auto read = [&](int ks) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < TNH; ++t) b[ks & 1][h][t] = fb.read(ws + ((ks >> 1) * 2 + h) * kNarrowF * kRowB, t, ks & 1);
+      };
+      {
+        read(0);
+        if (ahead) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          if (ks + 1 < KS) read(ks + 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < TNH; ++t)
+#pragma unroll
+              for (int i = 0; i < TM; ++i) acc[h][t][i] = mma16<E>(x[i][ks], b[ks & 1][h][t], ks ? acc[h][t][i] : c0[h][t]);
+          if constexpr (decltype(last)::value) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) x[i][ks] = load_x(rn, i, ks);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      const int pitch = (int)g.ldo * 2, vo = 4 * q * pitch + (n0 + c) * 2;
+      const int rows = (int)(g.M - mt < kNarrowRows ? g.M - mt : kNarrowRows) - 4 * q;
+      if (full)
+        narrow_rows<O, ACT, true>(acc, ro, vo, pitch, rows, 2);
+      else
+        narrow_rows<O, ACT, false>(acc, ro, vo, pitch, rows, g.N - n0 - c);
+    };
+    for (int sgi = 0; sgi < SG - 1; ++sgi) group(sgi, std::false_type{});
+    group(SG - 1, std::true_type{});
+  }
+}
+
 // ---- host side of one operand type
 struct FwdCall {
   const void *x, *wg, *wu;
@@ -692,18 +871,18 @@ struct Tiling {
 constexpr Tiling kTilings[3] = {{256, 128, 4, 2, 1, {1.8, 7.8, 2.0}, 6.0},
                                 {128, 64, 2, 2, 2, {0.98, 3.9, 1.1}, 3.7},
                                 {64, 32, 2, 2, 4, {0.75, 2.05, 0.9}, 2.0}};
-constexpr double kStageMin = 0.5, kSplitUs = 5.0, kBytesPerUs = 4e6;
+constexpr double kStageMin = 0.8, kSplitUs = 5.0, kBytesPerUs = 8e6;
 
 struct Plan {
   int tiling, splits;
   int64_t kps;
+  double us;
 };
 
 // rows x cols outputs of `groups` products with `segs` sums of K; wide: a tile is 2 * bnh columns (else the
 // two blocks are Wg's and Wu's); outputs: fp32 values of one partial
 inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bool wide, int es, int64_t outputs) {
-  Plan best{0, 1, K};
-  double least = 1e300;
+  Plan best{0, 1, K, 1e300};
   const int64_t bke = kRowB / es, stages = cdiv(K, bke);
   for (int c = 0; c < 3; ++c) {
     const Tiling& t = kTilings[c];
@@ -716,15 +895,23 @@ inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bo
       const double us = (double)(n / slots) * ((double)(per * segs) * ts + t.ends) +
                         (n % slots ? (double)(per * segs) * part + t.ends : 0.0) +
                         (s > 1 ? kSplitUs + 8.0 * (double)outputs * (double)s / kBytesPerUs : 0.0);
-      if (us < least) {
-        least = us;
-        best = Plan{c, (int)cdiv(stages, per), s > 1 ? per * bke : K};
-      }
+      if (us < best.us) best = Plan{c, (int)cdiv(stages, per), s > 1 ? per * bke : K, us};
     }
   }
   return best;
 }
 inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
+// narrow rows (16-bit forward): rounds of 8 waves' tiles in each work-group, 14 (k of 256 bytes) or 15.5 us a
+// round as measured (60000 x 512: D = 128 30 us against 40, 256 49 against 55), where that is less
+inline int64_t narrow_groups(int64_t M, int64_t F, int64_t kbytes) {
+  return std::max<int64_t>(1, std::min<int64_t>(256 / cdiv(F, kNarrowF), cdiv(cdiv(M, narrow_rows_of(kbytes)), 8)));
+}
+inline bool take_narrow(int64_t M, int64_t D, int64_t F) {
+  const int64_t kbytes = 2 * D;
+  if (kbytes > kNarrowBytes) return false;
+  const int64_t groups = narrow_groups(M, F, kbytes), rounds = cdiv(cdiv(M, narrow_rows_of(kbytes)), 8 * groups);
+  return cdiv(F, kNarrowF) <= 256 && 2.0 + (kbytes <= 256 ? 14.0 : 15.5) * (double)rounds < plan_gated(M, D, F, 2).us;
+}
 inline Plan plan_dx(int64_t M, int64_t D, int64_t F, int es) { return plan(M, D, F, 2, 1, true, es, M * D); }
 inline Plan plan_dw(int64_t M, int64_t D, int64_t F, int es) { return plan(F, D, M, 1, 2, true, es, 2 * F * D); }
 
@@ -738,8 +925,9 @@ inline int64_t part_floats(int64_t M, int64_t D, int64_t F, int es, bool bwd) {
   }
   return n;
 }
-// rows of bias partials: one for each wave's rows of a tile, or for 64 rows where k is split
-constexpr int kFinishRows = 64;
+// rows of bias partials: one for each wave's rows of a tile, or for 16 rows where k is split (few rows a
+// work-group: the splits' values are fetched one row after the other)
+constexpr int kFinishRows = 16;
 inline int64_t bias_parts(int64_t M, const Plan& p) {
   return p.splits > 1 ? cdiv(M, kFinishRows) : cdiv(M, kTilings[p.tiling].bm) * kTilings[p.tiling].wm;
 }
@@ -770,6 +958,20 @@ template <class E, class O, bool NMN, bool MMN, int EPI, int ACT>
 int launch(GemmArgs& g, int tiling, hipStream_t s) {
   if (tiling == 0 && EPI != EPI_RAW) return launch_tiling<E, O, NMN, MMN, EPI, ACT, EPI == EPI_RAW ? 1 : 0>(g, s);
   return tiling == 1 ? launch_tiling<E, O, NMN, MMN, EPI, ACT, 1>(g, s) : launch_tiling<E, O, NMN, MMN, EPI, ACT, 2>(g, s);
+}
+template <class E, class O, int ACT>
+int launch_narrow(GemmArgs& g, hipStream_t s) {
+  g.tiles_n = (int)cdiv(g.N, kNarrowF);
+  g.tiles_m = (int)narrow_groups(g.M, g.N, g.K * elem_size<E>());
+  g.ntiles = g.tiles_n * g.tiles_m;
+  g.per_xcd = (int)cdiv(g.ntiles, 8);
+  const dim3 grid((unsigned)(g.per_xcd * 8));
+  if (g.K * elem_size<E>() <= 256)
+    hipLaunchKernelGGL((narrow_kernel<E, O, ACT, 4>), grid, dim3(512), 0, s, g);
+  else
+    hipLaunchKernelGGL((narrow_kernel<E, O, ACT, 8>), grid, dim3(512), 0, s, g);
+  PCST_LAUNCH_CHECK("gated_linear");
+  return PCST_OK;
 }
 template <class E, class O, int EPI>
 int launch_act(GemmArgs& g, int tiling, int act, hipStream_t s) {
@@ -809,7 +1011,7 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a) {
     float g = 0.0f, u = 0.0f;
     if (in) {
       const float* p = a.part + m * a.F + f;
-#pragma unroll 4
+#pragma unroll 8
       for (int k = 0; k < a.splits; ++k) {
         g += p[2 * k * n];
         u += p[(2 * k + 1) * n];
@@ -909,6 +1111,12 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
     return c.act == ACT_SILU   ? launch_rows<E, O, ACT_SILU>(g, s)
            : c.act == ACT_GELU ? launch_rows<E, O, ACT_GELU>(g, s)
                                : launch_rows<E, O, ACT_RELU>(g, s);
+  if constexpr (elem_size<E>() == 2) {
+    if (take_narrow(c.M, c.D, c.F))
+      return c.act == ACT_SILU   ? launch_narrow<E, O, ACT_SILU>(g, s)
+             : c.act == ACT_GELU ? launch_narrow<E, O, ACT_GELU>(g, s)
+                                 : launch_narrow<E, O, ACT_RELU>(g, s);
+  }
   return run_gated<E, O, EPI_FWD>(g, plan_gated(c.M, c.D, c.F, elem_size<E>()), c.act, c.part, s);
 }
 
