@@ -3,11 +3,15 @@ defaults and order), so pickled configs in reference checkpoints map onto it and
 field the hot path reads (feature_dim, time_embed_dim, global_points, num_timesteps, schedule,
 cond_drop_prob, lambda_chamfer, use_amp, use_hierarchical, ...) means the same thing.
 
-Three additions, keyword fields with defaults that keep the reference behaviour:
+Five additions, keyword fields with defaults that keep the reference behaviour:
 `precision` ("fp32": exact-f32 MFMA, the parity default; "bf16": bf16 MFMA perf mode of the
-noise MLP, what bench.py measures),
+noise MLP, what bench.py measures; "fp8", gated blocks only: their gate and up products on e4m3
+operands, the rest bf16),
 `amp_dtype` (the 16-bit operand format of the training GEMMs under `use_amp`: "float16", the
-reference's CUDA autocast default, trainer.py:50,78, or "bfloat16"; same MFMA rate) and
+reference's CUDA autocast default, trainer.py:50,78, or "bfloat16"; same MFMA rate),
+`noise_block` ("relu": the reference's six residual blocks; "gated": pre-norm gated ones, models/blocks.py,
+with parameters of their own names), `fused_clip` (True: the trainer clips with utils.clip_grad_norm_ on a
+GPU, same norm and coefficient up to the order of the sum) and
 `make_dirs` (the reference creates log/result/checkpoint directories in the CWD on
 construction, config.py:64-67; set False to skip)."""
 from dataclasses import dataclass
@@ -74,6 +78,8 @@ class Config:
     precision: str = "fp32"
     amp_dtype: str = "float16"
     make_dirs: bool = True
+    noise_block: str = "relu"
+    fused_clip: bool = False
 
     def __post_init__(self):
         if not self.make_dirs:
@@ -83,6 +89,7 @@ class Config:
             os.makedirs(d, exist_ok=True)
 
     def __setstate__(self, state):
-        # reference pickles carry no `precision` / `amp_dtype` / `make_dirs`: fill the defaults
-        self.__dict__.update({"precision": "fp32", "amp_dtype": "float16", "make_dirs": True})
+        # reference pickles carry none of the additions: fill the defaults
+        self.__dict__.update({"precision": "fp32", "amp_dtype": "float16", "make_dirs": True,
+                              "noise_block": "relu", "fused_clip": False})
         self.__dict__.update(state)

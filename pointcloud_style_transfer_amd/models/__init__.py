@@ -8,6 +8,7 @@ from .diffusion_model import (
     DiffusionProcess,
 )
 from .blocks import (
+    GatedBlock,
     GatedLinear,
     RMSNorm,
     gated_linear,
@@ -30,6 +31,7 @@ __all__ = [
     "PointNet2Encoder",
     "RMSNorm",
     "GatedLinear",
+    "GatedBlock",
     "rms_norm",
     "rms_norm_quant",
     "quant_rows",

@@ -97,3 +97,41 @@ class GatedLinear(nn.Module):
 
     def forward(self, x):
         return gated_linear(x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias, self.act)
+
+
+class GatedBlock(nn.Module):
+    """A pre-norm gated residual block on (x, delta), delta the previous block's output:
+    s = x + delta; forward -> (s, Dropout(Linear(GatedLinear(RMSNorm(s)))))."""
+
+    def __init__(self, dim: int, hidden: int, act: str = "silu", dropout: float = 0.1):
+        super().__init__()
+        self.norm = RMSNorm(dim)
+        self.ff = GatedLinear(dim, hidden, act)
+        self.down = nn.Linear(hidden, dim)
+        self.drop = nn.Dropout(dropout)
+
+    def forward(self, x, delta=None):
+        n, s = (self.norm(x), x) if delta is None else self.norm(x, delta)
+        return s, self.drop(_ag.linear(self.ff(n), self.down))
+
+    @torch.no_grad()
+    def pack(self, eight: bool):
+        """The weights as `infer` reads them: bfloat16, gate and up in 8 bits with their scales if `eight`."""
+        ff = self.ff
+        gate, up = ((quant_rows(w.detach()) if eight else (w.detach().to(torch.bfloat16),))
+                    for w in (ff.gate.weight, ff.up.weight))
+        return (self.norm.weight.detach().float(), (*gate, *up, ff.gate.bias.detach().float(), ff.up.bias.detach().float()),
+                self.down.weight.detach().to(torch.bfloat16), self.down.bias.detach().float(), eight)
+
+    @torch.no_grad()
+    def infer(self, packed, x, delta=None):
+        """forward without dropout and gradients on bfloat16 rows x, delta [M, dim]; packed: pack()."""
+        w, ff, down, bias, eight = packed
+        if eight:
+            q, scale, *s = rms_norm_quant(x, w, delta, self.norm.eps)
+            s = s[0] if s else x
+            h = gated_linear_quant(q, scale, *ff, self.ff.act)
+        else:
+            n, s = (rms_norm(x, w, None, self.norm.eps), x) if delta is None else rms_norm(x, w, delta, self.norm.eps)
+            h = _hip.gated_linear(n, *ff, self.ff.act)
+        return s, _hip.gemm_ex(h, down, bias, epilogue=_hip.EP_BF16)

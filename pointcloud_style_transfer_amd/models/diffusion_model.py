@@ -29,6 +29,7 @@ from .. import packing
 from .. import rng as _rng
 from ..config.config import Config
 from . import _autograd as _ag
+from .blocks import GatedBlock, RMSNorm, rms_norm
 from .pointnet2_encoder import PointNet2Encoder
 
 
@@ -97,9 +98,16 @@ class NoisePredictor(nn.Module):
         self.time_embedding = TimeEmbedding(config.time_embed_dim)
         self.time_proj = nn.Linear(config.time_embed_dim, fd)
         self.style_proj = nn.Linear(fd, fd)
-        self.layers = nn.ModuleList([
-            nn.Sequential(nn.Linear(fd, fd * 2), nn.ReLU(), nn.Linear(fd * 2, fd), nn.Dropout(0.1))
-            for _ in range(6)])
+        self.gated = getattr(config, "noise_block", "relu") == "gated"
+        if not self.gated and getattr(config, "noise_block", "relu") != "relu":
+            raise ValueError(f"Config.noise_block must be 'relu' or 'gated', got {config.noise_block!r}")
+        if self.gated:
+            self.layers = nn.ModuleList([GatedBlock(fd, fd * 2, dropout=0.1) for _ in range(6)])
+            self.out_norm = RMSNorm(fd)
+        else:
+            self.layers = nn.ModuleList([
+                nn.Sequential(nn.Linear(fd, fd * 2), nn.ReLU(), nn.Linear(fd * 2, fd), nn.Dropout(0.1))
+                for _ in range(6)])
         self.output_mlp = nn.Sequential(nn.Linear(fd, 256), nn.ReLU(), nn.Linear(256, 128),
                                         nn.ReLU(), nn.Linear(128, 3))
         self._pack_key = None
@@ -110,13 +118,18 @@ class NoisePredictor(nn.Module):
         """ABI precision code: "bf16" runs the bf16 (solo) kernel, "fp32" the exact-f32 parity
         kernel."""
         p = getattr(self.config, "precision", "fp32")
+        if p == "fp8" and not self.gated:
+            raise ValueError("Config.precision 'fp8' is for gated blocks (Config.noise_block)")
         return packing.BF16 if p == "bf16" else packing.F32
 
     def packed(self):
         """Packed MFMA weight stream + bias table, rebuilt when any weight changes."""
         params = list(self.parameters())
         dev = params[0].device
-        key = (self.precision_code, str(dev), tuple((p.data_ptr(), p._version) for p in params))
+        key = (getattr(self.config, "precision", "fp32") if self.gated else self.precision_code, str(dev),
+               tuple((p.data_ptr(), p._version) for p in params))
+        if key != self._pack_key and self.gated:
+            self._packed, self._pack_key = self._pack_gated(key[0]), key
         if key != self._pack_key:
             sd = {f"noise_predictor.{k}": v.detach().float().cpu().numpy()
                   for k, v in self.state_dict().items()}
@@ -148,7 +161,35 @@ class NoisePredictor(nn.Module):
         return out
 
     def _dropout_active(self) -> bool:
-        return self.training and any(l[3].p > 0 for l in self.layers)
+        return self.training and any((l.drop if self.gated else l[3]).p > 0 for l in self.layers)
+
+    def _pack_gated(self, precision):
+        """What _infer_gated reads: None in fp32 (the autograd path's kernels on the parameters)."""
+        if precision not in ("bf16", "fp8"):
+            return None
+        pe, om = self.point_encoder, self.output_mlp
+        w0 = F.pad(pe[0].weight.detach().float(), (0, 5))  # K = 3 padded to 8, as the points are
+        lins = [(w0.to(torch.bfloat16), pe[0].bias.detach().float())]
+        lins += [(m.weight.detach().to(torch.bfloat16), m.bias.detach().float())
+                 for m in (pe[2], pe[4], om[0], om[2], om[4])]
+        return lins, [b.pack(precision == "fp8") for b in self.layers], self.out_norm.weight.detach().float()
+
+    def _infer_gated(self, noisy_points, timestep, style_feat):
+        """The gated network on bfloat16 rows: 16-bit products, the stream kept in 16 bits."""
+        lins, blocks, w_out = self.packed()
+        B, N, _ = noisy_points.shape
+        cond = torch.stack([_linear(self.time_embedding(timestep.to(noisy_points.device)), self.time_proj, False),
+                            _linear(style_feat.float(), self.style_proj, False)], 1)
+        lin = lambda x, k, ep, **kw: _hip.gemm_ex(x, *lins[k], epilogue=ep, **kw)  # noqa: E731
+        x = F.pad(noisy_points.reshape(B * N, 3).float(), (0, 5)).to(torch.bfloat16)
+        x = lin(lin(x, 0, _hip.EP_BF16, relu=True), 1, _hip.EP_BF16, relu=True)
+        x = lin(x, 2, _hip.EP_COND, aux=cond, group_rows=N, copy_bf16=True, fp32_out=False)
+        delta = None
+        for block, packed in zip(self.layers, blocks):
+            x, delta = block.infer(packed, x, delta)
+        x = rms_norm(x, w_out, delta, self.out_norm.eps)[0]
+        x = lin(lin(x, 3, _hip.EP_BF16, relu=True), 4, _hip.EP_BF16, relu=True)
+        return lin(x, 5, _hip.EP_F32).view(B, N, 3)
 
     def _forward_autograd(self, noisy_points, timestep, style_feat):
         """Differentiable path (training): every linear on the MFMA GEMM kernel with its
@@ -156,7 +197,7 @@ class NoisePredictor(nn.Module):
         pe = self.point_encoder
         tf = _ag.linear(self.time_embedding(timestep.to(noisy_points.device)), self.time_proj)
         sf = _ag.linear(style_feat, self.style_proj)
-        if noisy_points.is_cuda and torch.is_autocast_enabled("cuda"):
+        if not self.gated and noisy_points.is_cuda and torch.is_autocast_enabled("cuda"):
             # the whole per-point network on the 16-bit-storage fused GEMMs (NoisePredictorFn,
             # autocast's dtype);
             # each residual block keeps its own Dropout rate
@@ -168,7 +209,12 @@ class NoisePredictor(nn.Module):
         h = _ag.linear(h, pe[2], True)
         pf = _ag.linear(h, pe[4])
         x = pf + tf.unsqueeze(1) + sf.unsqueeze(1)
-        for layer in self.layers:
+        if self.gated:
+            delta = None
+            for layer in self.layers:
+                x, delta = layer(x, delta)
+            x = self.out_norm(x, delta)[0]
+        for layer in () if self.gated else self.layers:
             d = _ag.linear(_ag.linear(x, layer[0], True), layer[2])
             x = layer[3](d) + x
         h = _ag.linear(x, self.output_mlp[0], True)
@@ -176,9 +222,12 @@ class NoisePredictor(nn.Module):
         return _ag.linear(h, self.output_mlp[4])
 
     def fused_inference(self, style_feat: torch.Tensor) -> bool:
-        """True when forward() runs the fused inference kernel (no autograd, no dropout)."""
+        """True when forward() runs the fused inference kernel (no autograd, no dropout, no gated blocks)."""
+        return not self.gated and self._plain(style_feat)
+
+    def _plain(self, *inputs) -> bool:
         return not (_ag.needs_grad(self) or self._dropout_active()
-                    or (style_feat.requires_grad and torch.is_grad_enabled()))
+                    or (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)))
 
     def forward_cond(self, noisy_points: torch.Tensor, cond: torch.Tensor,
                      packed: Optional[tuple] = None, wait=None, signal=None) -> torch.Tensor:
@@ -197,6 +246,8 @@ class NoisePredictor(nn.Module):
     def forward(self, noisy_points: torch.Tensor, timestep: torch.Tensor,
                 style_feat: torch.Tensor) -> torch.Tensor:
         if not self.fused_inference(style_feat):
+            if self.gated and self._plain(noisy_points, style_feat) and self.packed() is not None:
+                return self._infer_gated(noisy_points, timestep, style_feat)
             return self._forward_autograd(noisy_points, timestep, style_feat)
         cond = self.cond(timestep.to(noisy_points.device), style_feat)
         return self.forward_cond(noisy_points, cond)

@@ -69,8 +69,8 @@ class DiffusionInference:
     """`DiffusionInference` (inference.py:62-171)."""
 
     def __init__(self, checkpoint_path: str, device: str = "cuda", *, precision: str = None):
-        if precision not in (None, "fp32", "bf16"):
-            raise ValueError(f"precision must be 'fp32' or 'bf16', got {precision!r}")
+        if precision not in (None, "fp32", "bf16", "fp8"):
+            raise ValueError(f"precision must be 'fp32', 'bf16' or 'fp8', got {precision!r}")
         dev = torch.device(device)
         if dev.type != "cuda":
             raise RuntimeError(f"DiffusionInference runs on the MI355X HIP path only; device "
@@ -154,9 +154,10 @@ def main(argv=None):
     p.add_argument("--visualize", action="store_true")
     p.add_argument("--num_steps", type=int, default=50)
     p.add_argument("--guidance_scale", type=float, default=7.5)
-    p.add_argument("--precision", choices=["fp32", "bf16"], default=None,
+    p.add_argument("--precision", choices=["fp32", "bf16", "fp8"], default=None,
                    help="noise-MLP arithmetic: fp32 (exact, the default of a reference "
-                        "checkpoint) or bf16 (the bf16 MFMA kernel bench.py measures)")
+                        "checkpoint), bf16 (the bf16 MFMA kernel bench.py measures) or fp8 (models "
+                        "with gated blocks)")
     args = p.parse_args(argv)
     try:
         eng = DiffusionInference(args.checkpoint, args.device, precision=args.precision)

@@ -46,6 +46,7 @@ from ..models.diffusion_model import DiffusionProcess, PointCloudDiffusionModel
 from ..models.losses import DiffusionLoss
 from ..utils.checkpoint import CheckpointManager
 from ..utils.ema import ExponentialMovingAverage
+from ..utils.grad_clip import clip_grad_norm_
 from ..utils.logger import Logger
 
 try:  # trainer.py:5 -- optional here
@@ -168,6 +169,7 @@ class DiffusionTrainer:
         self.max_patience = 20
         self.gradient_accumulation_steps = config.gradient_accumulation_steps
         self.gradient_clip_norm = 1.0
+        self.fused_clip = getattr(config, "fused_clip", False) and self.device_type == "cuda"
         self.ddp_model = self.model
         # train_step(next_batch=...): the next batch's style geometry (condition-cloud downsample,
         # FPS, ball query: positions only) is queued on a side stream at the start of a step and
@@ -220,7 +222,10 @@ class DiffusionTrainer:
             loss, terms = self._forward_backward(batch, geo)
         if sync:
             self.scaler.unscale_(self.optimizer)
-            torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.gradient_clip_norm)
+            if self.fused_clip:  # three launches, whatever the number of tensors
+                clip_grad_norm_(self.model.parameters(), self.gradient_clip_norm)
+            else:
+                torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.gradient_clip_norm)
             self.scaler.step(self.optimizer)
             self.scaler.update()
             self.optimizer.zero_grad()

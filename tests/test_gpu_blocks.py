@@ -584,6 +584,7 @@ def test_blocks_together():
     x, target = rand(1, 500, 96), rand(2, 500, 96, scale=50)
     loss, grads = run_blocks(blocks, x, target)
     want_loss, want = run_blocks(plain, x.double(), target.double())
+    loss, want_loss = loss.detach(), want_loss.detach()
     assert abs(float(loss) - float(want_loss)) < 1e-5 * float(want_loss)
     for g, w in zip(grads, want):
         assert float((g.double() - w).norm()) < 1e-4 * float(w.norm())
