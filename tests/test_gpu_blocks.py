@@ -304,6 +304,52 @@ def test_gated_large_tiles():
         check_grads(x, wg, wu, None, None, "silu", dh, _hip.gated_linear_bwd(x, wg, wu, dh), dtype)
 
 
+# many rows of few columns (the weights stay in LDS), rows, columns and k that end inside a tile
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("M,D,F", [(9000, 130, 999), (30000, 200, 301), (20011, 72, 701), (24577, 128, 640), (20000, 256, 512),
+                                   (40001, 33, 1000), (17000, 255, 385)])
+def test_gated_narrow(M, D, F, dtype):
+    act, bt = ["silu", "gelu", "relu"][F % 3], F32 if D % 2 else dtype
+    x, k = rand(1, M, D, dtype=dtype), D ** -0.5
+    wg, wu = rand(2, F, D, dtype=dtype, scale=k), rand(3, F, D, dtype=dtype, scale=k)
+    for bg, bu in ((rand(4, F, dtype=bt), rand(5, F, dtype=bt)), (None, None)):
+        h = _hip.gated_linear(x, wg, wu, bg, bu, act)
+        check_h(h, *gated_ref(x, wg, wu, bg, bu, act), act, dtype)
+    # a row's value does not depend on the rows beside it, whichever wave takes it
+    keep = [0, 47, 48, 63, 64, 4095, M - 2, M - 1]
+    y = torch.zeros_like(x)
+    y[keep] = x[keep]
+    assert torch.equal(_hip.gated_linear(y, wg, wu, act=act)[keep], h[keep])
+    shifted = torch.empty(x.numel() + 1, device="cuda", dtype=dtype)[1:].view_as(x).copy_(x)
+    assert torch.equal(_hip.gated_linear(shifted, wg, wu, act=act), h)
+    y = x.clone()
+    y[5] = math.inf
+    other = _hip.gated_linear(y, wg, wu, act=act)
+    assert torch.equal(other[6:], h[6:]) and torch.equal(other[:5], h[:5])
+
+
+# few tiles and a long k, which is split: in h (long D), in dx (long F), in dW (many rows)
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,D,F", [(65, 4000, 70), (100, 2999, 301), (300, 2000, 40), (70, 1000, 33), (5000, 65, 701),
+                                   (9000, 64, 1000), (700, 520, 200), (2000, 1030, 72)])
+def test_gated_splits(M, D, F, dtype):
+    act = ["silu", "gelu", "relu"][M % 3]
+    x, k = rand(1, M, D, dtype=dtype), D ** -0.5
+    wg, wu = rand(2, F, D, dtype=dtype, scale=k), rand(3, F, D, dtype=dtype, scale=k)
+    bt = F32 if F % 2 else dtype
+    bg, bu, dh = rand(4, F, dtype=bt), rand(5, F, dtype=bt), rand(6, M, F, dtype=dtype)
+    h = _hip.gated_linear(x, wg, wu, bg, bu, act)
+    check_h(h, *gated_ref(x, wg, wu, bg, bu, act), act, dtype)
+    grads = _hip.gated_linear_bwd(x, wg, wu, dh, bg, bu, act)
+    check_grads(x, wg, wu, bg, bu, act, dh, grads, dtype)
+    for a, b in zip(grads, _hip.gated_linear_bwd(x, wg, wu, dh, bg, bu, act)):
+        assert torch.equal(a, b)
+    assert torch.equal(h, _hip.gated_linear(x, wg, wu, bg, bu, act))
+    need = (1, 0, 0, 0, 1)
+    for n, a, b in zip(need, grads, _hip.gated_linear_bwd(x, wg, wu, dh, bg, bu, act, need=need)):
+        assert torch.equal(a, b) if n else b is None
+
+
 def test_gated_against_differences():
     M, D, F = 3, 9, 7
     x, wg, wu, bg, bu = rand(1, M, D), rand(2, F, D), rand(3, F, D), rand(4, F), rand(5, F)
@@ -339,7 +385,8 @@ def test_gated_needed_gradients(need):
 
 @pytest.mark.parametrize("out", [BF, F16])
 @pytest.mark.parametrize("M,D,F,bias", [(1, 16, 16, True), (3, 5, 7, False), (65, 130, 70, True), (200, 256, 300, False),
-                                        (140, 1000, 129, True), (6500, 256, 1100, False)])
+                                        (140, 1000, 129, True), (6500, 256, 1100, False), (70, 4000, 40, True),
+                                        (300, 2050, 65, False)])
 def test_gated_quant(M, D, F, bias, out):
     x, k = rand(1, M, D, dtype=BF), D ** -0.5
     q, xs = rms_norm_quant(x, torch.ones(D, device="cuda"))
