@@ -266,8 +266,42 @@ __device__ __forceinline__ void gated_rows(const GemmArgs& g, const f32x4 (&acc)
   constexpr int ES = elem_size<E>();
   constexpr bool FAST = ES < 4;
   const int n = g.N - f;
+  // dh's rows are fetched AHEAD row tiles before their use, rows past the end as the last one: with each row's
+  // load in front of its use, half of the epilogue is waiting
+  typedef Vec<O, TNH> V;
+  constexpr int AHEAD = EPI != EPI_BWD ? 1 : ES == 4 ? (TM < 2 ? TM : 2) : TM;
+  typename V::V dv[AHEAD][4];
+  auto fetch = [&](int i) {
+    const O* dh = static_cast<const O*>(g.dh) + f;
+    if (n >= TNH) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t m = m0 + 16 * i + r;
+        dv[i % AHEAD][r] = *reinterpret_cast<const typename V::Any*>(dh + (m < g.M ? m : g.M - 1) * g.N);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t m = m0 + 16 * i + r;
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) dv[i % AHEAD][r][t] = t < n ? dh[(m < g.M ? m : g.M - 1) * g.N + t] : (O)0.0f;
+      }
+    }
+  };
+  if (EPI == EPI_BWD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(i);
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
+    float d[4][TNH];
+    if (EPI == EPI_BWD) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) d[r][t] = (float)dv[i % AHEAD][r][t];
+      if (i + AHEAD < TM) fetch(i + AHEAD);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t m = m0 + 16 * i + r;
@@ -291,14 +325,13 @@ __device__ __forceinline__ void gated_rows(const GemmArgs& g, const f32x4 (&acc)
         for (int t = 0; t < TNH; ++t) o[t] = act_value<FAST, ACT>(gv[t]) * uv[t];
         if (n > 0) store_n<O, TNH>(static_cast<O*>(g.out[0]) + m * g.ldo + f, n, o);
       } else if (f < g.fpad) {
-        float d[TNH], og[TNH], ou[TNH];
-        load_bias<O, TNH>(g.dh, 0, m * g.N + f, n, d);
+        float og[TNH], ou[TNH];
 #pragma unroll
         for (int t = 0; t < TNH; ++t) {
           float v;
           const float da = act_grad<FAST, ACT>(gv[t], v);
-          og[t] = t < n ? d[t] * uv[t] * da : 0.0f;  // the padding up to fpad is zero
-          ou[t] = t < n ? d[t] * v : 0.0f;
+          og[t] = t < n ? d[r][t] * uv[t] * da : 0.0f;  // the padding up to fpad is zero
+          ou[t] = t < n ? d[r][t] * v : 0.0f;
           cg[t] += og[t];
           cu[t] += ou[t];
         }
@@ -1120,41 +1153,56 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
   return run_gated<E, O, EPI_FWD>(g, plan_gated(c.M, c.D, c.F, elem_size<E>()), c.act, c.part, s);
 }
 
-// dW's partials (one of n values per split and matrix) added in order; blockIdx.y: the matrix
-template <class O>
-__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, int64_t n, int parts,
-                                                      O* __restrict__ out0, O* __restrict__ out1) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= n) return;
-  part += blockIdx.y * n + e;
-  float s = 0.0f;
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * gridDim.y * n];
-  (blockIdx.y ? out1 : out0)[e] = (O)s;
-}
-// 16 columns a work-group, 16 slices of the parts
-template <class O>
-__global__ __launch_bounds__(256) void bias_kernel(const float* __restrict__ part, int F, int parts, O* dbg, O* dbu) {
+// Bias gradients from the row blocks' partials [parts, 2, F]: 16 columns a work-group, 16 slices of the parts
+struct BiasArgs {
+  const float* part;
+  int F, parts, f32;
+  void *dbg, *dbu;
+};
+template <class T>
+__device__ __forceinline__ void bias_columns(const BiasArgs& b, int block) {
   __shared__ double red[16][17];
   const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int f = blockIdx.x * 16 + c;  // of 2 F
+  const int f = block * 16 + c;  // of 2 F
   double s = 0.0;
-  if (f < 2 * F) {
+  if (f < 2 * b.F) {
 #pragma unroll 8
-    for (int p = q; p < parts; p += 16) s += (double)part[(int64_t)p * 2 * F + f];
+    for (int p = q; p < b.parts; p += 16) s += (double)b.part[(int64_t)p * 2 * b.F + f];
   }
   red[q][c] = s;
   __syncthreads();
-  if (q == 0 && f < 2 * F) {
+  if (q == 0 && f < 2 * b.F) {
     for (int i = 1; i < 16; ++i) s += red[i][c];
-    O* o = f < F ? dbg : dbu;
-    if (o) o[f < F ? f : f - F] = (O)(float)s;
+    void* o = f < b.F ? b.dbg : b.dbu;
+    const int at = f < b.F ? f : f - b.F;
+    if (o && b.f32) static_cast<float*>(o)[at] = (float)s;
+    else if (o) static_cast<T*>(o)[at] = (T)(float)s;
   }
+}
+template <class T>
+__global__ __launch_bounds__(256) void bias_kernel(BiasArgs b) {
+  bias_columns<T>(b, blockIdx.x);
+}
+// A product's partials (n values per split and group) added in order; `blocks` work-groups for each group and, in front
+// of them, the bias gradients, which would take a launch of their own (4.4 us, whatever their number)
+template <class O, class T>
+__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ part, int64_t n, int parts, int blocks,
+                                                      int groups, O* __restrict__ out0, O* __restrict__ out1, BiasArgs b) {
+  const int at = (int)blockIdx.x - ((int)gridDim.x - blocks * groups);
+  if (at < 0) return bias_columns<T>(b, blockIdx.x);
+  const int grp = at >= blocks;
+  const int64_t e = (int64_t)(at - grp * blocks) * 256 + threadIdx.x;
+  if (e >= n) return;
+  part += grp * n + e;
+  float s = 0.0f;
+#pragma unroll 16
+  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * groups * n];
+  (grp ? out1 : out0)[e] = (O)s;
 }
 
 // a plain product (dx, or dWg and dWu as two groups), over splits of k where the plan has them
 template <class E, class O, bool NMN, bool MMN>
-int run_product(GemmArgs& g, const Plan& p, float* part, hipStream_t s) {
+int run_product(GemmArgs& g, const Plan& p, float* part, const BiasArgs& b, hipStream_t s) {
   if (p.splits == 1) return launch<E, O, NMN, MMN, EPI_OUT, 0>(g, p.tiling, s);
   const int64_t n = g.M * g.N;
   O *o0 = static_cast<O*>(g.out[0]), *o1 = static_cast<O*>(g.out[1]);
@@ -1164,8 +1212,9 @@ int run_product(GemmArgs& g, const Plan& p, float* part, hipStream_t s) {
   g.out[1] = part + n;
   g.o_split = g.groups * n;
   if (int rc = launch<E, float, NMN, MMN, EPI_OUT, 0>(g, p.tiling, s)) return rc;
-  hipLaunchKernelGGL(combine_kernel<O>, dim3((unsigned)cdiv(n, 256), (unsigned)g.groups), dim3(256), 0, s, part, n,
-                     p.splits, o0, o1);
+  const int blocks = (int)cdiv(n, 256), front = b.part ? (int)cdiv(2 * b.F, 16) : 0;
+  hipLaunchKernelGGL((combine_kernel<O, typename E::T>), dim3((unsigned)(blocks * g.groups + front)), dim3(256), 0, s, part,
+                     n, p.splits, blocks, g.groups, o0, o1, b);
   PCST_LAUNCH_CHECK("gated_linear_bwd");
   return PCST_OK;
 }
@@ -1184,15 +1233,10 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   const Plan pg = plan_gated(f.M, f.D, f.F, ES);
   int rc = run_gated<E, T, EPI_BWD>(g, pg, f.act, f.part, s);
   if (rc) return rc;
-  if (g.bpart) {
-    const dim3 grid((unsigned)cdiv(2 * f.F, 16));
-    const int parts = (int)bias_parts(f.M, pg);
-    if (c.bgrad_f32)
-      hipLaunchKernelGGL(bias_kernel<float>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts,
-                         static_cast<float*>(c.dbg), static_cast<float*>(c.dbu));
-    else
-      hipLaunchKernelGGL(bias_kernel<T>, grid, dim3(256), 0, s, c.bpart, (int)f.F, parts, static_cast<T*>(c.dbg),
-                         static_cast<T*>(c.dbu));
+  BiasArgs bias{g.bpart, (int)f.F, (int)bias_parts(f.M, pg), c.bgrad_f32, c.dbg, c.dbu};
+  const Plan pw = plan_dw(f.M, f.D, f.F, ES);
+  if (bias.part && (pw.splits == 1 || !(c.dwg || c.dwu))) {  // no work-groups of dW's to go with
+    hipLaunchKernelGGL(bias_kernel<T>, dim3((unsigned)cdiv(2 * f.F, 16)), dim3(256), 0, s, bias);
     PCST_LAUNCH_CHECK("gated_linear_bwd");
   }
   if (c.dx) {
@@ -1210,11 +1254,10 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.out[0] = c.dx;
     d.ldo = f.D;
     const Plan p = plan_dx(f.M, f.D, f.F, ES);
-    rc = run_product<E, T, true, false>(d, p, f.part, s);
+    rc = run_product<E, T, true, false>(d, p, f.part, BiasArgs{}, s);
     if (rc) return rc;
   }
   if (c.dwg || c.dwu) {
-    const Plan p = plan_dw(f.M, f.D, f.F, ES);
     GemmArgs w{};
     w.a[0] = static_cast<const char*>(c.dgu);
     w.b0[0] = static_cast<const char*>(f.x);
@@ -1231,7 +1274,8 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
         w.a_group[w.groups] = k * c.fpad * ES;
         w.out[w.groups++] = outs[k];
       }
-    rc = c.wgrad_f32 ? run_product<E, float, true, true>(w, p, f.part, s) : run_product<E, T, true, true>(w, p, f.part, s);
+    rc = c.wgrad_f32 ? run_product<E, float, true, true>(w, pw, f.part, bias, s)
+                     : run_product<E, T, true, true>(w, pw, f.part, bias, s);
     if (rc) return rc;
   }
   return PCST_OK;
