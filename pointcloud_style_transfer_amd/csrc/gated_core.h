@@ -729,13 +729,16 @@ __global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
 }
 
 // ---- narrow rows (K of at most 512 bytes, many rows): a work-group keeps 128 features of both matrices in
-// LDS for its whole life, and each of its waves takes tiles of 64 rows by itself, straight from memory into
+// LDS for its whole life, and each of its waves takes tiles of 64 or 32 rows by itself, straight from memory into
 // registers: no barrier after the start, so that one wave's epilogue runs beside the other's products, and
 // x is read once for every 128 features instead of W once for every 256 rows.  The next tile's rows are
 // loaded as this one's are used for the last time.
 constexpr int kNarrowF = 128, kNarrowBytes = 512;
-// rows of a wave's tile: what the registers hold of x beside the sums
-__host__ __device__ constexpr int narrow_rows_of(int64_t kbytes) { return kbytes <= 256 ? 64 : 48; }
+// Rows of a wave's tile: what the registers hold of x beside the sums, of two groups of features where the outputs
+// of one are made between the products of the next (x 256: 120000 rows 79 -> 75 us, 30000 27 -> 23 for the smaller
+// tiles; x 128: no gain from it, so the larger tile).  Tiles go to the waves so that a SIMD's two waves differ
+// where the number is no whole one (60000 x 256 x 512: 50 -> 42 us).
+__host__ __device__ constexpr int narrow_rows_of(int64_t kbytes) { return kbytes <= 256 ? 64 : 32; }
 
 // The forward's epilogue of narrow_kernel (whose sums hold the biases): 2 features of a 16-bit output,
 // addressed with 32 bits from the tile's first row (vo: the lane's offset; a row's is scalar).  FULL: all rows,
@@ -766,6 +769,7 @@ template <class E, class O, int ACT, int KS>
 __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   constexpr int ES = elem_size<E>(), kNarrowRows = narrow_rows_of(KS * 64), TM = kNarrowRows / 16, TNH = 2;
   constexpr int IM = KS / 2, SG = kNarrowF / 32;
+  constexpr bool PIPED = KS == 8;
   __shared__ __attribute__((aligned(1024))) char lds_w[IM * 2 * kNarrowF * kRowB];
   __shared__ float lds_b[2][kNarrowF];                                   // biases
   // tiles_n blocks of features x tiles_m groups of rows; an XCD's work-groups share row groups
@@ -804,7 +808,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   // 4-byte accesses of pairs of features: all 128 there, and rows on 4-byte boundaries
   const bool whole = n0 + kNarrowF <= g.N && (g.N & 1) == 0 && ((uintptr_t)g.out[0] & 3) == 0;
   const int step = g.tiles_m * 8, tiles = (int)((g.M + kNarrowRows - 1) / kNarrowRows);
-  int tile = rg * 8 + wave;
+  int tile = wave * g.tiles_m + rg;
   auto tile_rsrc = [&](int t) {
     const int64_t m0 = (int64_t)t * kNarrowRows, rows = g.M - m0 < kNarrowRows ? g.M - m0 : kNarrowRows;
     return make_rsrc(g.a[0] + m0 * g.lda, t < tiles ? (int)(rows * g.lda) : 0);  // past the last tile: fetches nothing
@@ -823,6 +827,73 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+
+  // A whole tile: a group's outputs are made between the products of the next one, a few instructions behind
+  // each, so that the matrix unit and the others work at the same time in every wave.
+  auto piped = [&](rsrc_t ro, rsrc_t rn) {
+    if constexpr (PIPED) {
+    typedef typename Vec<O, 2>::V V2;
+    constexpr int NP = TM * 4;  // pieces of a group's epilogue: 2 features of a row
+    const int pitch = (int)g.ldo * 2;
+    f32x4 acc[2][2][TNH][TM];
+    auto piece = [&](int sgi, int p) {
+      const int i = p / 4, row = 16 * i + p % 4;
+      V2 o;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        o[t] = (O)(act_value<true, ACT>(acc[sgi & 1][0][t][i][p % 4]) * acc[sgi & 1][1][t][i][p % 4]);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, o), ro, 4 * q * pitch + (n0 + sgi * 32 + l * TNH) * 2,
+                                            row * pitch, 0);
+    };
+#pragma unroll
+    for (int sgi = 0; sgi < SG; ++sgi) {
+      const PCST_LDS char* ws = w + sgi * 32 * kRowB;
+      i32x4 b[2][2][TNH];
+      auto read = [&](int ks) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < TNH; ++t) b[ks & 1][h][t] = fb.read(ws + ((ks >> 1) * 2 + h) * kNarrowF * kRowB, t, ks & 1);
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < TNH; ++t) {
+          const float v = lds_b[h][sgi * 32 + l * TNH + t];
+#pragma unroll
+          for (int i = 0; i < TM; ++i) acc[sgi & 1][h][t][i] = f32x4{v, v, v, v};
+        }
+      read(0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) read(ks + 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < TNH; ++t)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+              acc[sgi & 1][h][t][i] = mma16<E>(x[i][ks], b[ks & 1][h][t], acc[sgi & 1][h][t][i]);
+        if (sgi) {
+#pragma unroll
+          for (int p = ks * NP / KS; p < (ks + 1) * NP / KS; ++p) piece(sgi - 1, p);
+        }
+        if (sgi == SG - 1) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) x[i][ks] = load_x(rn, i, ks);
+        }
+#pragma unroll
+        for (int n = 0; n < 4 * TM; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                        // an MFMA,
+          __builtin_amdgcn_sched_group_barrier(0x002, ACT == ACT_GELU ? 6 : 3, 0);  // what runs beside it
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) piece(SG - 1, p);
+    }
+  };
 
   for (; tile < tiles; tile += step) {
     const int64_t mt = (int64_t)tile * kNarrowRows;
@@ -870,11 +941,15 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
       __builtin_amdgcn_s_setprio(0);
       const int pitch = (int)g.ldo * 2, vo = 4 * q * pitch + (n0 + c) * 2;
       const int rows = (int)(g.M - mt < kNarrowRows ? g.M - mt : kNarrowRows) - 4 * q;
-      if (full)
+      if (!PIPED && full)
         narrow_rows<O, ACT, true>(acc, ro, vo, pitch, rows, 2);
       else
         narrow_rows<O, ACT, false>(acc, ro, vo, pitch, rows, g.N - n0 - c);
     };
+    if (PIPED && full) {
+      piped(ro, rn);
+      continue;
+    }
     for (int sgi = 0; sgi < SG - 1; ++sgi) group(sgi, std::false_type{});
     group(SG - 1, std::true_type{});
   }
@@ -943,16 +1018,16 @@ inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bo
   return best;
 }
 inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
-// narrow rows (16-bit forward): rounds of 8 waves' tiles in each work-group, 14 (k of 256 bytes) or 15.5 us a
-// round as measured (60000 x 512: D = 128 30 us against 40, 256 49 against 55), where that is less
+// narrow rows (16-bit forward): taken where 5 us and 1.13 (k of 256 bytes: 1.57) for each tile of a CU, as measured
+// (us; 60000 x 512: D = 128 28 against 40 for the tiles above, 256 42 against 55), are less than the tiles' estimate
 inline int64_t narrow_groups(int64_t M, int64_t F, int64_t kbytes) {
   return std::max<int64_t>(1, std::min<int64_t>(256 / cdiv(F, kNarrowF), cdiv(cdiv(M, narrow_rows_of(kbytes)), 8)));
 }
 inline bool take_narrow(int64_t M, int64_t D, int64_t F) {
   const int64_t kbytes = 2 * D;
-  if (kbytes > kNarrowBytes) return false;
-  const int64_t groups = narrow_groups(M, F, kbytes), rounds = cdiv(cdiv(M, narrow_rows_of(kbytes)), 8 * groups);
-  return cdiv(F, kNarrowF) <= 256 && 2.0 + (kbytes <= 256 ? 14.0 : 15.5) * (double)rounds < plan_gated(M, D, F, 2).us;
+  if (kbytes > kNarrowBytes || cdiv(F, kNarrowF) > 256) return false;
+  const int64_t each = cdiv(cdiv(M, narrow_rows_of(kbytes)), narrow_groups(M, F, kbytes));
+  return 5.0 + (kbytes <= 256 ? 1.57 : 1.13) * (double)each < plan_gated(M, D, F, 2).us;
 }
 inline Plan plan_dx(int64_t M, int64_t D, int64_t F, int es) { return plan(M, D, F, 2, 1, true, es, M * D); }
 inline Plan plan_dw(int64_t M, int64_t D, int64_t F, int es) { return plan(F, D, M, 1, 2, true, es, 2 * F * D); }
