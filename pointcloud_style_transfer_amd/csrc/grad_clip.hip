@@ -5,10 +5,11 @@
 //
 // Two launches (per 128 tensors): the norm's, whose work-groups each leave one partial in fp64, and
 // the scaling's, whose work-groups each add all partials in the same fixed order themselves -- at most
-// 1024 a launch, so that no third launch, no atomic and no zeroed counter stands between.  fp64 sums: a square of any finite float is finite there, and the order does not show in the
-// 24 bits returned.  The tensors' addresses travel in the kernel arguments, so a captured launch keeps
-// them.  Bound by HBM: every gradient is read twice and written once.
+// 1024 a launch, so that no third launch, no atomic and no zeroed counter stands between.  fp64 sums: a
+// square of any finite float is finite there, and their order does not show in the 24 bits returned.  The
+// tensors' addresses travel in the kernel arguments, so a captured launch keeps them.  Bound by HBM: every gradient is read twice and written once.
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -66,6 +67,25 @@ __device__ __forceinline__ double add_term(double s, float v, int p) {
   return p == 2 ? fma(d, d, s) : p == 1 ? s + fabs(d) : nan_max(s, fabs(d));
 }
 
+// 8 values.  A 16-bit value's square is exact in fp32: four of them are added there, two roundings of 2^-24 of
+// their sum, and fp64 adds the fours (268M fp16, whose norm waits for fp64's instructions: 382 -> 357 us).
+// bf16 squares may leave fp32's range on either side; such fours go the way of fp32's values.
+template <class V>
+__device__ __forceinline__ double add_piece(double s, V v, int p) {
+  constexpr bool kF = std::is_same<V, Vec<_Float16, 8>::V>::value, kB = std::is_same<V, Vec<__bf16, 8>::V>::value;
+#pragma unroll
+  for (int j = 0; j < 8; j += 4) {
+    const float a = (float)v[j], b = (float)v[j + 1], c = (float)v[j + 2], d = (float)v[j + 3];
+    const float q = fmaf(b, b, a * a) + fmaf(d, d, c * c);
+    if ((kF || kB) && p == 2 && (kF || (q > 0x1p-100f && q < 0x1p120f))) {
+      s += (double)q;
+    } else {
+      s = add_term(add_term(add_term(add_term(s, a, p), b, p), c, p), d, p);
+    }
+  }
+  return s;
+}
+
 constexpr int kFlight = 4;  // 8-value pieces a thread has in flight
 
 template <class T>
@@ -77,9 +97,7 @@ __device__ __forceinline__ double range_sum(const T* g, int64_t lo, int64_t hi, 
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) v[u] = *reinterpret_cast<const typename Vec<T, 8>::Any*>(g + i + u * 2048);
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s = add_term(s, (float)v[u][j], p);
+    for (int u = 0; u < kFlight; ++u) s = add_piece(s, v[u], p);
   }
   for (; i < hi; i += 2048) {
     float v[8];

@@ -549,6 +549,20 @@ def test_clip_counts(count, n):
     check_clip(grads, before, norm, grads, 1.0, 2)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_clip_range(dtype):
+    """Values whose squares underflow or overflow fp32 (bf16), in the same groups as others; fp16's whole range."""
+    tiny, huge = (2.0 ** -120, 2.0 ** 100) if dtype == BF else (2.0 ** -24, 2.0 ** 15)
+    for top in (1.0, tiny, huge):
+        g = rand(1, 50_000, dtype=F32).abs().clamp(0.5, 1.5)
+        g = torch.where(torch.arange(50_000, device="cuda") % 7 == 3, g * top, g * tiny).to(dtype)
+        n = float(g.double().square().sum().sqrt())
+        assert abs(float(clip_grads([g.clone()], math.inf)) - n) <= 2 * R * n
+    g = torch.zeros(50_000, device="cuda", dtype=dtype)
+    g[9] = tiny
+    assert float(clip_grads([g], math.inf)) == tiny
+
+
 def test_clip_as_torch_does():
     params = [torch.nn.Parameter(rand(i, *s)) for i, s in enumerate([(64, 32), (64,), (3, 5, 7), (1,)])]
     for scale in (1e-4, 1.0):
