@@ -521,7 +521,7 @@ int pcst_rms_norm_bwd(const void* s, int dtype, int64_t M, int64_t D, const void
  * (erf), 2 relu.  PCST_E4M3 operands carry a scale for each row (x_scale [M], gate_scale, up_scale
  * [F]) and give out_dtype PCST_BF16 or PCST_F16, their biases are of that or float; elsewhere out_dtype = dtype and the scales are NULL.
  * Products accumulate in fp32, h is rounded once.  workspace: pcst_gated_linear_workspace_size bytes (0 for
- * M <= 64), for the partial sums of products that split D, and for copies of operands where D * element
+ * M <= 16), for the partial sums of products that split D, and for copies of operands where D * element
  * size is no multiple of 16 or aligned does not say that x, Wg and Wu start on 16-byte boundaries. */
 int pcst_gated_linear_workspace_size(int dtype, int64_t M, int64_t D, int64_t F, int aligned, size_t* bytes);
 int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D, const void* w_gate,

@@ -1482,7 +1482,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=Non
     h = torch.empty(M, F, dtype=out_dtype, device=x.device)
     dt = _ELEM[x.dtype]
     ws = None
-    if M > 64:  # (fewer rows need none)
+    if M > 16:  # (fewer rows need none)
         aligned = (x.data_ptr() | w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
         ws = _workspace("pcst_gated_linear_workspace_size", dt, M, D, F, int(aligned), device=x.device)
     _call("pcst_gated_linear", _addr(x), dt, M, D, _addr(w_gate), _addr(w_up), F, _addr(b_gate), _addr(b_up),

@@ -634,31 +634,31 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 ? 4 : 2) void gemm_kernel(Ge
   } while (LOOP && more);
 }
 
-// ---- few rows (M <= 64): the weights are read once, straight into the MFMA's registers.  A work-group owns
+// ---- few rows (at most 128, see take_rows): the weights are read once, straight into the MFMA's registers.  A work-group owns
 // 16 features of both matrices; its 8 waves split k and add up in LDS, in order.  Bound by reading the weights
-// (and, at a handful of rows, by the launch).  Rows may start at any element: no copies.
+// (and, at a handful of rows, by the launch: 1 x 1024 x 2816 bf16 4.8 us for 11.5 MB).  Rows may start at any element: no copies.
+// 16 bytes of a row from `off` on, zeros past its end: where it ends inside, the row's last 16 moved down
 template <class E>
 __device__ __forceinline__ i32x4 piece16(const char* row, int64_t off, int64_t bytes) {
   typedef Vec<typename E::T, 16 / elem_size<E>()> V;
-  if (off + 16 <= bytes)
-    return __builtin_bit_cast(i32x4, (typename V::V)*reinterpret_cast<const typename V::Any*>(row + off));
-  i32x4 v{0, 0, 0, 0};
-#pragma unroll
-  for (int b = 0; b < 16; b += elem_size<E>())
-    if (off + b < bytes) {
-      const uint32_t w = elem_size<E>() == 4   ? *reinterpret_cast<const uint32_t*>(row + off + b)
-                         : elem_size<E>() == 2 ? *reinterpret_cast<const uint16_t*>(row + off + b)
-                                               : *reinterpret_cast<const uint8_t*>(row + off + b);
-      v[b / 4] |= (int)(w << (8 * (b & 3)));
-    }
-  return v;
+  if (off >= bytes) return i32x4{0, 0, 0, 0};
+  const int64_t at = off + 16 <= bytes ? off : bytes - 16;
+  if (at < 0) {  // (rows of less than 16 bytes)
+    i32x4 v{0, 0, 0, 0};
+#pragma unroll 1
+    for (int b = 0; b < (int)bytes; ++b) v[b >> 2] |= (int)((uint32_t)(uint8_t)row[b] << (8 * (b & 3)));
+    return v;
+  }
+  const i32x4 v = __builtin_bit_cast(i32x4, (typename V::V)*reinterpret_cast<const typename V::Any*>(row + at));
+  const int n = (int)(off - at);  // bytes in front
+  if (n == 0) return v;
+  const unsigned __int128 w = __builtin_bit_cast(unsigned __int128, v) >> (8 * n);
+  return __builtin_bit_cast(i32x4, w);
 }
-
-constexpr int kRowsMax = 64;
 
 template <class E, class O, int ACT, int TM>
 __global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
-  constexpr int ES = elem_size<E>(), P = ES == 1 ? 2 : 1, U = TM == 4 ? 2 : 4;  // pieces a product, products in flight
+  constexpr int ES = elem_size<E>(), P = ES == 1 ? 2 : 1, U = TM == 8 ? 1 : TM == 4 ? 2 : 4;  // pieces a product, products in flight
   __shared__ f32x4 red[8][2][TM][64];
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -674,20 +674,29 @@ __global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
   f32x4 acc[2][TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) acc[0][i] = acc[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; s += U) {
-    i32x4 a[U][TM][P], b[U][2][P];
+  // UN steps at once; CHECK: a piece may end behind its row
+  auto products = [&](int s, auto un, auto check) {
+    constexpr int UN = decltype(un)::value;
+    typedef Vec<typename E::T, 16 / ES> V;
+    i32x4 a[UN][TM][P], b[UN][2][P];
+    auto piece = [&](const char* row, int64_t off) {
+      if constexpr (decltype(check)::value)
+        return piece16<E>(row, off, bytes);
+      else
+        return __builtin_bit_cast(i32x4, (typename V::V)*reinterpret_cast<const typename V::Any*>(row + off));
+    };
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const int64_t off = s + u < s1 ? ((int64_t)(s + u) * P + p) * 64 + q * 16 : bytes;
-        b[u][0][p] = piece16<E>(wg, off, bytes);
-        b[u][1][p] = piece16<E>(wu, off, bytes);
+        const int64_t off = ((int64_t)(s + u) * P + p) * 64 + q * 16;
+        b[u][0][p] = piece(wg, off);
+        b[u][1][p] = piece(wu, off);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[u][i][p] = piece16<E>(x[i], off, bytes);
+        for (int i = 0; i < TM; ++i) a[u][i][p] = piece(x[i], off);
       }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -697,7 +706,12 @@ __global__ __launch_bounds__(512) void rows_kernel(GemmArgs g) {
           else
             acc[h][i] = mma16<E>(a[u][i][0], b[u][h][0], acc[h][i]);
         }
-  }
+  };
+  const int whole = (int)(bytes / (64 * P)) < s1 ? (int)(bytes / (64 * P)) : s1;
+  int s = s0;
+  for (; s + U <= whole; s += U) products(s, std::integral_constant<int, U>{}, std::false_type{});
+  for (; s < whole; ++s) products(s, std::integral_constant<int, 1>{}, std::false_type{});
+  if (s < s1) products(s, std::integral_constant<int, 1>{}, std::true_type{});
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -976,7 +990,12 @@ struct BwdCall {
 };
 
 // ---- which tiles, and over how many splits of k
-// Tiles of 256 x 2*128, 128 x 2*64 and 64 x 2*32; 1, 2 and 4 work-groups of them run on a CU.  The time of a
+// Tiles of 256 x 2*128, 128 x 2*64 and 64 x 2*32; 1, 2 and 4 work-groups of them run on a CU.  With the device full
+// the largest reach 1.17 PFLOP/s (8192 x 4096 x 8192 bf16, 936 us; a plain product of this size in the library 1.33)
+// and 2.2 to 2.4 in e4m3 (465 to 505 us; 2.85), the matrix units busy in 61 % of the cycles.  What bounds them is
+// power: waves that take turns at reading and multiplying, over half-length stages, kept them busy in 69 % of
+// 11 % fewer cycles, and the clock fell from 1.83 to 1.67 GHz (912 us, shorter sums slower).  float: 138 TFLOP/s of 152.
+// The time of a
 // launch is estimated as rounds of work-groups x (stages x a stage's time + a tile's start and end), both
 // measured with the device full (us, 16-bit: 8192 x 4096 x 8192; start and end: 60000 x 512 with k = 64 .. 512);
 // a round that leaves CUs with fewer work-groups is faster by that, down to the latency of a load.  Splitting
@@ -1028,6 +1047,17 @@ inline bool take_narrow(int64_t M, int64_t D, int64_t F) {
   if (kbytes > kNarrowBytes || cdiv(F, kNarrowF) > 256) return false;
   const int64_t each = cdiv(cdiv(M, narrow_rows_of(kbytes)), narrow_groups(M, F, kbytes));
   return 5.0 + (kbytes <= 256 ? 1.57 : 1.13) * (double)each < plan_gated(M, D, F, 2).us;
+}
+// few rows: always up to 16 (no workspace to ask for), up to 128 where 3.5 us and 0.45 + 0.19 for each 16 rows of x
+// per 512 bytes of k and 256 work-groups are less than the tiles' estimate, the launch that adds their splits
+// and the copies of ragged rows.  Measured (us, bf16): 1024 x 2816: 16 rows 5.5 against 9.3 for tiles, 64 8.6 against
+// 13.9, 4096 x 1000: 13.1 against 14.6, 24.3 against 14.6; 1001 x 3000: 15.6 against 28 at 64 rows.
+constexpr int kRowsFew = 16, kRowsMax = 128;
+inline bool take_rows(int64_t M, int64_t D, int64_t F, int es) {
+  if (M <= kRowsFew || M > kRowsMax) return M <= kRowsFew;
+  const double tm = M <= 32 ? 2.0 : M <= 64 ? 4.0 : es == 4 ? 12.0 : 10.0;  // (from 65 rows on one work-group a CU)
+  const double rows = 3.5 + (0.45 + 0.19 * tm) * (double)cdiv(D * es, 512) * std::max(1.0, (double)F / 4096.0);
+  return rows < plan_gated(M, D, F, es).us + 2.5 + (D * es % 16 ? 12.0 : 0.0);
 }
 inline Plan plan_dx(int64_t M, int64_t D, int64_t F, int es) { return plan(M, D, F, 2, 1, true, es, M * D); }
 inline Plan plan_dw(int64_t M, int64_t D, int64_t F, int es) { return plan(F, D, M, 1, 2, true, es, 2 * F * D); }
@@ -1124,15 +1154,38 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs a) {
     load_bias<O, 1>(a.bg, a.bias_f32, f, 1, bg);
     load_bias<O, 1>(a.bu, a.bias_f32, f, 1, bu);
   }
-  for (int64_t m = m0 + w; m < m0 + kFinishRows && m < a.M; m += 4) {
-    float g = 0.0f, u = 0.0f;
-    if (in) {
-      const float* p = a.part + m * a.F + f;
-#pragma unroll 8
-      for (int k = 0; k < a.splits; ++k) {
-        g += p[2 * k * n];
-        u += p[(2 * k + 1) * n];
+  // a wave's rows and eight splits at a time in flight, whatever their number: past the end the last one again, unused
+  constexpr int R = kFinishRows / 4;
+  float gs[R], us[R];
+  const float* p[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int64_t m = m0 + w + 4 * j;
+    p[j] = a.part + (m < a.M ? m : a.M - 1) * a.F + (in ? f : a.F - 1);
+    gs[j] = us[j] = 0.0f;
+  }
+  for (int k0 = 0; k0 < a.splits; k0 += 8) {
+    float v[8][R][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[k][j][h] = p[j][(2 * (int64_t)(k0 + k < a.splits ? k0 + k : a.splits - 1) + h) * n];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        gs[j] += k0 + k < a.splits ? v[k][j][0] : 0.0f;
+        us[j] += k0 + k < a.splits ? v[k][j][1] : 0.0f;
       }
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int64_t m = m0 + w + 4 * j;
+    if (m >= a.M) continue;
+    float g = gs[j], u = us[j];
+    if (in) {
       if (elem_size<E>() == 1) {
         g *= a.xs[m] * a.gs[f];
         u *= a.xs[m] * a.us[f];
@@ -1214,7 +1267,8 @@ int launch_rows(const GemmArgs& g, hipStream_t s) {
   const dim3 grid((unsigned)cdiv(g.N, 16));
   if (g.M <= 16) hipLaunchKernelGGL((rows_kernel<E, O, ACT, 1>), grid, dim3(512), 0, s, g);
   else if (g.M <= 32) hipLaunchKernelGGL((rows_kernel<E, O, ACT, 2>), grid, dim3(512), 0, s, g);
-  else hipLaunchKernelGGL((rows_kernel<E, O, ACT, 4>), grid, dim3(512), 0, s, g);
+  else if (g.M <= 64) hipLaunchKernelGGL((rows_kernel<E, O, ACT, 4>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((rows_kernel<E, O, ACT, 8>), grid, dim3(512), 0, s, g);
   PCST_LAUNCH_CHECK("gated_linear");
   return PCST_OK;
 }
@@ -1224,7 +1278,7 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
   GemmArgs g = fwd_args(c);
   g.out[0] = c.h;
   g.ldo = c.F;
-  if (c.M <= kRowsMax)
+  if (take_rows(c.M, c.D, c.F, elem_size<E>()))
     return c.act == ACT_SILU   ? launch_rows<E, O, ACT_SILU>(g, s)
            : c.act == ACT_GELU ? launch_rows<E, O, ACT_GELU>(g, s)
                                : launch_rows<E, O, ACT_RELU>(g, s);
@@ -1250,8 +1304,13 @@ __device__ __forceinline__ void bias_columns(const BiasArgs& b, int block) {
   const int f = block * 16 + c;  // of 2 F
   double s = 0.0;
   if (f < 2 * b.F) {
-#pragma unroll 8
-    for (int p = q; p < b.parts; p += 16) s += (double)b.part[(int64_t)p * 2 * b.F + f];
+    for (int p0 = q; p0 < b.parts; p0 += 16 * 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = b.part[(int64_t)(p0 + 16 * k < b.parts ? p0 + 16 * k : p0) * 2 * b.F + f];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += p0 + 16 * k < b.parts ? (double)v[k] : 0.0;
+    }
   }
   red[q][c] = s;
   __syncthreads();
@@ -1279,8 +1338,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
   if (e >= n) return;
   part += grp * n + e;
   float s = 0.0f;
-#pragma unroll 16
-  for (int p = 0; p < parts; ++p) s += part[(int64_t)p * groups * n];
+  for (int p0 = 0; p0 < parts; p0 += 16) {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = part[(int64_t)(p0 + k < parts ? p0 + k : p0) * groups * n];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += p0 + k < parts ? v[k] : 0.0f;
+  }
   (grp ? out1 : out0)[e] = (O)s;
 }
 
@@ -1319,7 +1383,9 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   if (rc) return rc;
   BiasArgs bias{g.bpart, (int)f.F, (int)bias_parts(f.M, pg), c.bgrad_f32, c.dbg, c.dbu};
   const Plan pw = plan_dw(f.M, f.D, f.F, ES);
-  if (bias.part && (pw.splits == 1 || !(c.dwg || c.dwu))) {  // no work-groups of dW's to go with
+  const Plan px = plan_dx(f.M, f.D, f.F, ES);
+  const bool with_dx = c.dx && px.splits > 1, with_dw = !with_dx && (c.dwg || c.dwu) && pw.splits > 1;
+  if (bias.part && !with_dx && !with_dw) {  // no adding of splits to go with
     hipLaunchKernelGGL(bias_kernel<T>, dim3((unsigned)cdiv(2 * f.F, 16)), dim3(256), 0, s, bias);
     PCST_LAUNCH_CHECK("gated_linear_bwd");
   }
@@ -1337,8 +1403,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
     d.splits = d.groups = 1;
     d.out[0] = c.dx;
     d.ldo = f.D;
-    const Plan p = plan_dx(f.M, f.D, f.F, ES);
-    rc = run_product<E, T, true, false>(d, p, f.part, BiasArgs{}, s);
+    rc = run_product<E, T, true, false>(d, px, f.part, with_dx ? bias : BiasArgs{}, s);
     if (rc) return rc;
   }
   if (c.dwg || c.dwu) {
@@ -1358,6 +1423,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
         w.a_group[w.groups] = k * c.fpad * ES;
         w.out[w.groups++] = outs[k];
       }
+    if (!with_dw) bias = BiasArgs{};
     rc = c.wgrad_f32 ? run_product<E, float, true, true>(w, pw, f.part, bias, s)
                      : run_product<E, T, true, true>(w, pw, f.part, bias, s);
     if (rc) return rc;

@@ -106,7 +106,7 @@ extern "C" int pcst_gated_linear_workspace_size(int dtype, int64_t M, int64_t D,
   if (int rc = check("gated_linear_workspace_size", dtype, M, D, F, 0)) return rc;
   PCST_CHECK_ARG(bytes, "gated_linear_workspace_size: null pointer");
   const bool pad = !aligned || (D * elem(dtype)) % 16 != 0;
-  *bytes = M <= gated::kRowsMax ? 0 : lay(nullptr, dtype, M, D, F, pad, false).bytes;
+  *bytes = gated::take_rows(M, D, F, elem(dtype)) ? 0 : lay(nullptr, dtype, M, D, F, pad, false).bytes;
   return PCST_OK;
 }
 
@@ -126,7 +126,7 @@ extern "C" int pcst_gated_linear(const void* x, int dtype, int64_t M, int64_t D,
   if (M == 0) return PCST_OK;
   PCST_CHECK_ARG(x && w_gate && w_up && h, "gated_linear: null pointer");
   const int es = elem(dtype);
-  const bool rows = M <= gated::kRowsMax;
+  const bool rows = gated::take_rows(M, D, F, es);
   const bool pad = !ready(x, D, es) || !ready(w_gate, D, es) || !ready(w_up, D, es);
   const Layout l = lay(workspace, dtype, M, D, F, pad, false);
   PCST_CHECK_ARG(rows || l.bytes == 0 || workspace, "gated_linear: null workspace");

@@ -55,8 +55,8 @@ def test_norm_null_pointers_and_no_rows():
     (dict(D=0), EINVAL), (dict(F=0), EINVAL), (dict(M=-1), EINVAL), (dict(D=1 << 20), EUNSUPPORTED),
     (dict(F=1 << 20), EUNSUPPORTED), (dict(M=1 << 31), EUNSUPPORTED), (dict(dt=4), EINVAL), (dict(act=3), EINVAL),
     (dict(out=2), EINVAL), (dict(dt=3, out=1), EINVAL), (dict(dt=3, out=0), EINVAL), (dict(bg=16), EINVAL), (dict(x=None), EINVAL),
-    (dict(D=9, M=65), EINVAL), (dict(x=24, M=65), EINVAL),  # rows off 16-byte boundaries, and no workspace
-    (dict(D=8192, M=65), EINVAL),  # a product that splits D, and no workspace
+    (dict(D=9, M=129), EINVAL), (dict(x=24, M=129), EINVAL),  # rows off 16-byte boundaries, and no workspace
+    (dict(D=8192, M=129), EINVAL),  # a product that splits D, and no workspace
 ])
 def test_gated_refusals(kw, want):
     a = dict(x=16, dt=1, M=4, D=8, F=8, bg=None, bu=None, act=0, out=1)
@@ -77,10 +77,10 @@ def test_gated_bwd_refusals():
     assert call(dt=3) == EINVAL and call(M=0) == EINVAL and call(ws=None) == EINVAL
     assert call(dh=None) == EINVAL and call(bg=one) == EINVAL
     assert size("pcst_gated_linear_bwd_workspace_size", 3, 4, 8, 8)[0] == EINVAL
-    assert size("pcst_gated_linear_workspace_size", 1, 65, 64, 8, 1) == (0, 0)
+    assert size("pcst_gated_linear_workspace_size", 1, 129, 64, 8, 1) == (0, 0)
     assert size("pcst_gated_linear_workspace_size", 1, 64, 63, 8, 0) == (0, 0)
-    assert size("pcst_gated_linear_workspace_size", 1, 65, 64, 8, 0)[1] > 0
-    assert size("pcst_gated_linear_workspace_size", 1, 65, 63, 8, 1)[1] > 0
+    assert size("pcst_gated_linear_workspace_size", 1, 129, 64, 8, 0)[1] > 0
+    assert size("pcst_gated_linear_workspace_size", 1, 129, 63, 8, 1)[1] > 0
     assert size("pcst_gated_linear_workspace_size", 1, 65, 8192, 8, 1)[1] > 0
     assert size("pcst_gated_linear_workspace_size", 1, 8192, 4096, 8192, 1) == (0, 0)
 

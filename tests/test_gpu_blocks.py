@@ -328,10 +328,36 @@ def test_gated_narrow(M, D, F, dtype):
     assert torch.equal(other[6:], h[6:]) and torch.equal(other[:5], h[:5])
 
 
+# 1 to 128 rows on either kernel, rows of every alignment, the last piece of a row of any length
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,D,F", [(1, 1, 3), (2, 3, 17), (17, 7, 16), (66, 31, 40), (100, 519, 130), (128, 1000, 64), (128, 4096, 48),
+                                   (97, 130, 300), (127, 2050, 33), (65, 64, 8)])
+def test_gated_few_rows(M, D, F, dtype):
+    act = ["silu", "gelu", "relu"][M % 3]
+    k = D ** -0.5
+    bx = torch.full((M * D + 40,), math.nan, device="cuda", dtype=dtype)
+    bw = torch.full((2 * F * D + 40,), math.nan, device="cuda", dtype=dtype)
+    for at in (0, 1, 8):  # elements in front; what lies around the operands is NaN
+        x, wg, wu = bx[at:at + M * D].view(M, D), bw[at:at + F * D].view(F, D), bw[at + F * D:at + 2 * F * D].view(F, D)
+        x.copy_(rand(1, M, D))
+        wg.copy_(rand(2, F, D, scale=k))
+        wu.copy_(rand(3, F, D, scale=k))
+        b = rand(4, F)
+        check_h(_hip.gated_linear(x, wg, wu, b, b, act), *gated_ref(x, wg, wu, b, b, act), act, dtype)
+        if dtype == BF:
+            (q, xs), (g8, gs), (u8, us) = quant_rows(x), quant_rows(wg), quant_rows(wu)
+            h = gated_linear_quant(q, xs, g8, gs, u8, us, b, b, act=act)
+            full = [torch.cat([t.view(torch.uint8), t.view(torch.uint8)[:1]]).view(torch.float8_e4m3fn)[:n] for t, n in ((q, M), (g8, F), (u8, F))]
+            assert torch.equal(h, gated_linear_quant(full[0], xs, full[1], gs, full[2], us, b, b, act=act))
+        bx.fill_(math.nan)
+        bw.fill_(math.nan)
+
+
 # few tiles and a long k, which is split: in h (long D), in dx (long F), in dW (many rows)
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("M,D,F", [(65, 4000, 70), (100, 2999, 301), (300, 2000, 40), (70, 1000, 33), (5000, 65, 701),
-                                   (9000, 64, 1000), (700, 520, 200), (2000, 1030, 72)])
+                                   (9000, 64, 1000), (700, 520, 200), (2000, 1030, 72),
+                                   (33, 4100, 5200)])
 def test_gated_splits(M, D, F, dtype):
     act = ["silu", "gelu", "relu"][M % 3]
     x, k = rand(1, M, D, dtype=dtype), D ** -0.5
