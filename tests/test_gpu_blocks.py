@@ -517,6 +517,19 @@ def test_gated_autocast():
         check_grads(*det, "silu", dh, rounded, half, wdtype=F32)
 
 
+def test_backward_on_either_thread():
+    x, wg, wu, w = rand(1, 300, 128, dtype=BF), rand(2, 96, 128, dtype=BF), rand(3, 96, 128, dtype=BF), rand(4, 128)
+    dh = rand(5, 300, 96, dtype=BF)
+    got = []
+    for threads in (False, True):
+        with torch.autograd.set_multithreading_enabled(threads):
+            leaves = [t.clone().requires_grad_() for t in (x, w, wg, wu)]
+            got.append(torch.autograd.grad(gated_linear(rms_norm(*leaves[:2]), *leaves[2:]), leaves, dh))
+    assert not torch._C._is_multithreading_enabled()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_deterministic():
     x, wg, wu, dh = rand(1, 3000, 128, dtype=BF), rand(2, 96, 128, dtype=BF), rand(3, 96, 128, dtype=BF), rand(4, 3000, 96, dtype=BF)
     b = rand(5, 96)
