@@ -5,7 +5,8 @@
     delta' = Linear(act(n Wg^T + bg) * (n Wu^T + bu))
 
 Functions first (rms_norm, gated_linear with gradients; rms_norm_quant, quant_rows, gated_linear_quant for
-serving in 8 bits), then the modules that hold their weights.
+serving in 8 bits), then the modules that hold their weights.  All may be captured into a HIP graph, a forward
+with its backward together; as torch has it, no eager graph of the same leaves may be alive at a capture.
 """
 from __future__ import annotations
 

@@ -767,6 +767,38 @@ def test_graph():
                 assert torch.equal(a, b)
 
 
+def test_graph_with_autograd():
+    """A block's forward and backward through autograd, captured, replayed between eager passes of the same leaves."""
+    torch.manual_seed(0)
+    block = Block(256, 512).cuda()
+    params = list(block.parameters())
+    x, d, dy = (rand(i, 2500, 256, dtype=F32) for i in (1, 2, 3))
+
+    def work():
+        with torch.autocast("cuda", dtype=F16):
+            s, o = block(x, d)
+        return [s.detach(), o.detach(), *torch.autograd.grad([s, o], params, [dy, dy.to(o.dtype)])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for k in range(4):
+        for i, t in enumerate((x, d, dy)):
+            t.copy_(rand(10 * k + i, 2500, 256))
+        with torch.no_grad():
+            block.ff.gate.weight.add_(0.01)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, work()):
+            assert torch.equal(a, b)
+
+
 def test_modules_train():
     """Gradients through the modules, in place into .grad, next to torch's own layers; no second derivatives."""
     block = Block(64, 96).cuda()
