@@ -178,6 +178,8 @@ def _stream():
 
 def _tensor_device_index(args, kwargs):
     """Device index of the first HIP tensor among the arguments (duck-typed), else None."""
+    if args and isinstance(args[0], torch.Tensor) and args[0].is_cuda:  # nearly every call
+        return args[0].get_device()
     for a in list(args) + list(kwargs.values()):
         if isinstance(a, (tuple, list)):  # knn3_query's (orig, idx, ws) handle
             for b in a:
@@ -1340,31 +1342,37 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _raw_stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+def _raw_stream(t):
+    """The current stream of t's device, which is the current one (_on_tensor_device)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _same_device(what, t, *others):
-    require_device(t, *others)
     d = t.get_device()
-    for o in others:
-        if o is not None and o.get_device() != d:
-            raise RuntimeError(f"{what}: tensors on different devices ({t.device}, {o.device})")
+    if d >= 0:
+        for o in others:
+            if o is not None and o.get_device() != d:
+                break
+        else:
+            return
+    require_device(t, *others)
+    raise RuntimeError(f"{what}: tensors on different devices ({[str(o.device) for o in (t, *others) if o is not None]})")
 
 
 def _norm_operands(what, x, weight, residual):
     """x, weight and residual of a row norm, checked: (x, weight, residual) contiguous, M, D."""
-    if x.dim() < 1 or x.dtype not in _FLOATS:
-        raise RuntimeError(f"{what}: x is a float32, bfloat16 or float16 tensor [..., D], got {x.dtype}")
-    D = x.shape[-1]
+    dtype, shape = x.dtype, x.shape
+    if not shape or dtype not in _FLOATS:
+        raise RuntimeError(f"{what}: x is a float32, bfloat16 or float16 tensor [..., D], got {dtype}")
+    D = shape[-1]
     if D == 0:
         raise RuntimeError(f"{what}: rows of no values")
     if weight is not None:
-        if tuple(weight.shape) != (D,) or weight.dtype not in (x.dtype, torch.float32):
+        if weight.shape != (D,) or (weight.dtype != dtype and weight.dtype != torch.float32):
             raise RuntimeError(f"{what}: weight is [{D}] of {x.dtype} or float32, got {weight.dtype} "
                                f"{list(weight.shape)}")
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        if residual.shape != shape or residual.dtype != dtype:
             raise RuntimeError(f"{what}: residual is {x.dtype} {list(x.shape)} like x, got "
                                f"{residual.dtype} {list(residual.shape)}")
     _same_device(what, x, weight, residual)
@@ -1379,9 +1387,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, stats=False):
     x, weight, residual, M, D = _norm_operands("rms_norm", x, weight, residual)
     y = torch.empty_like(x)
     s = x if residual is None else torch.empty_like(x)
-    rho = torch.empty(M, dtype=torch.float32, device=x.device) if stats else None
+    rho = x.new_empty(M, dtype=torch.float32) if stats else None
     _call("pcst_rms_norm", _addr(x), _addr(residual), _ELEM[x.dtype], M, D, _addr(weight),
-          _ELEM[weight.dtype], eps, _addr(y), _addr(s), _addr(rho), _raw_stream())
+          _ELEM[weight.dtype], eps, y.data_ptr(), s.data_ptr(), _addr(rho), _raw_stream(x))
     return y, s, rho
 
 
@@ -1401,7 +1409,7 @@ def rms_norm_bwd(s, weight, rho, dy, ds=None, need_dx=True, need_dw=True):
     dw = torch.empty_like(weight) if need_dw else None
     ws = _workspace("pcst_rms_norm_bwd_workspace_size", M, D, device=s.device) if need_dw else None
     _call("pcst_rms_norm_bwd", _addr(s), _ELEM[s.dtype], M, D, _addr(weight), _ELEM[weight.dtype],
-          _addr(rho), _addr(dy), _addr(ds), _addr(dx), _addr(dw), _addr(ws), _raw_stream())
+          _addr(rho), _addr(dy), _addr(ds), _addr(dx), _addr(dw), _addr(ws), _raw_stream(s))
     return dx, dw
 
 
@@ -1409,11 +1417,11 @@ def rms_norm_quant(x, weight, residual=None, eps=1e-6):
     """rms_norm with an 8-bit output -> (q float8_e4m3fn like x, scale float32 [rows], s):
     scale = max |y| / 448 over a row (1 for a row of zeros), q = y / scale rounded to nearest even."""
     x, weight, residual, M, D = _norm_operands("rms_norm_quant", x, weight, residual)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     s = x if residual is None else torch.empty_like(x)
     _call("pcst_rms_norm_quant", _addr(x), _addr(residual), _ELEM[x.dtype], M, D, _addr(weight),
-          _ELEM[weight.dtype], eps, _addr(q), _addr(scale), _addr(s), _raw_stream())
+          _ELEM[weight.dtype], eps, _addr(q), _addr(scale), _addr(s), _raw_stream(x))
     return q, scale, s
 
 
@@ -1421,29 +1429,31 @@ def quant_rows(x):
     """x [..., D] -> (q float8_e4m3fn like x, scale float32 [...]): rows in 8 bits, as
     rms_norm_quant's."""
     x, _, _, M, D = _norm_operands("quant_rows", x, None, None)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call("pcst_quant_rows", _addr(x), _ELEM[x.dtype], M, D, _addr(q), _addr(scale), _raw_stream())
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _call("pcst_quant_rows", _addr(x), _ELEM[x.dtype], M, D, _addr(q), _addr(scale), _raw_stream(x))
     return q, scale
 
 
 def _gated_operands(what, x, w_gate, w_up, b_gate, b_up, act, bias_dtype):
     if act not in ACTS:
         raise RuntimeError(f"{what}: act is one of {sorted(ACTS)}, got {act!r}")
-    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[1]:
+    xshape, wshape = x.shape, w_gate.shape
+    if len(xshape) != 2 or len(wshape) != 2 or wshape != w_up.shape or wshape[1] != xshape[1]:
         raise RuntimeError(f"{what}: shapes are x [M,D], w_gate and w_up [F,D], got {list(x.shape)}, "
                            f"{list(w_gate.shape)}, {list(w_up.shape)}")
-    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+    dtype = x.dtype
+    if w_gate.dtype != dtype or w_up.dtype != dtype:
         raise RuntimeError(f"{what}: x and the weights are of one type, got {x.dtype}, {w_gate.dtype}, "
                            f"{w_up.dtype}")
     if (b_gate is None) != (b_up is None):
         raise RuntimeError(f"{what}: both biases or none")
-    F = w_gate.shape[0]
+    F = wshape[0]
     if b_gate is not None:
         if tuple(b_gate.shape) != (F,) or tuple(b_up.shape) != (F,) or b_gate.dtype != b_up.dtype \
                 or b_gate.dtype not in (bias_dtype, torch.float32):
             raise RuntimeError(f"{what}: the biases are [{F}] of {bias_dtype} or float32")
-    if F == 0 or x.shape[1] == 0:
+    if F == 0 or xshape[1] == 0:
         raise RuntimeError(f"{what}: no features ({list(x.shape)}, {list(w_gate.shape)})")
     _same_device(what, x, w_gate, w_up, b_gate, b_up)
     if b_gate is not None:
@@ -1479,7 +1489,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=Non
                 raise RuntimeError("gated_linear: scales are float32, one for each row")
         _same_device("gated_linear", x, *scales)
         xs, gs, us = (t.contiguous() for t in scales)
-    h = torch.empty(M, F, dtype=out_dtype, device=x.device)
+    h = x.new_empty((M, F), dtype=out_dtype)
     dt = _ELEM[x.dtype]
     ws = None
     if M > 16:  # (fewer rows need none)
@@ -1487,7 +1497,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu", scales=Non
         ws = _workspace("pcst_gated_linear_workspace_size", dt, M, D, F, int(aligned), device=x.device)
     _call("pcst_gated_linear", _addr(x), dt, M, D, _addr(w_gate), _addr(w_up), F, _addr(b_gate), _addr(b_up),
           _bias_f32(b_gate), ACTS[act], _addr(xs), _addr(gs), _addr(us), _addr(h), _ELEM[out_dtype], _addr(ws),
-          _raw_stream())
+          _raw_stream(x))
     return h
 
 
@@ -1517,7 +1527,7 @@ def gated_linear_bwd(x, w_gate, w_up, dh, b_gate=None, b_up=None, act="silu", ne
         ws = _workspace("pcst_gated_linear_bwd_workspace_size", dt, M, D, F, device=dev)
         _call("pcst_gated_linear_bwd", _addr(x), dt, M, D, _addr(w_gate), _addr(w_up), F, _addr(b_gate),
               _addr(b_up), _bias_f32(b_gate), ACTS[act], _addr(dh), _addr(dx), _addr(dw[0]), _addr(dw[1]),
-              1 if wgrad_dtype == torch.float32 else 0, _addr(db[0]), _addr(db[1]), _addr(ws), _raw_stream())
+              1 if wgrad_dtype == torch.float32 else 0, _addr(db[0]), _addr(db[1]), _addr(ws), _raw_stream(x))
     return (dx, *dw, *db)
 
 
@@ -1606,7 +1616,7 @@ def grad_clip(grads, max_norm, norm_type=2.0, inv_scale=None, out=None, scale=Tr
     _call("pcst_grad_clip_workspace_size", sizes, n, ctypes.byref(sz))
     ws = torch.empty(sz.value, dtype=torch.uint8, device=dev)
     _call("pcst_grad_clip", ptr.buffer_info()[0], optr.buffer_info()[0] if scale else None, sizes, types, n, p,
-          max_norm, _addr(inv_scale), norm.data_ptr(), ws.data_ptr(), _raw_stream())
+          max_norm, _addr(inv_scale), norm.data_ptr(), ws.data_ptr(), _raw_stream(norm))
     if scale:  # what autograd saved of these tensors is now another value
         torch.autograd.graph.increment_version(grads if out is None else out)
     return norm
