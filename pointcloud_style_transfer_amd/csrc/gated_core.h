@@ -754,36 +754,57 @@ constexpr int kNarrowF = 128, kNarrowBytes = 512;
 // where the number is no whole one (60000 x 256 x 512: 50 -> 42 us).
 __host__ __device__ constexpr int narrow_rows_of(int64_t kbytes) { return kbytes <= 256 ? 64 : 32; }
 
-// The forward's epilogue of narrow_kernel (whose sums hold the biases): 2 features of a 16-bit output,
-// addressed with 32 bits from the tile's first row (vo: the lane's offset; a row's is scalar).  FULL: all rows,
-// both features and 4-byte stores; else each value by itself, behind its limits.
-template <class O, int ACT, bool FULL, int TM>
-__device__ __forceinline__ void narrow_rows(const f32x4 (&acc)[2][2][TM], rsrc_t out, int vo, int pitch, int rows, int n) {
-  typedef typename Vec<O, 2>::V V2;
+// narrow_kernel's accesses: 2 features of a 16-bit matrix, addressed with 32 bits from the tile's first row (vo: the
+// lane's offset; a row's is scalar).  FULL: both features and 4-byte accesses; else each value by itself, n of them.
+template <class O, bool FULL>
+__device__ __forceinline__ typename Vec<O, 2>::V narrow_load(rsrc_t from, int vo, int so, int n) {
+  typename Vec<O, 2>::V v{};
+  if (FULL) return __builtin_bit_cast(typename Vec<O, 2>::V, __builtin_amdgcn_raw_buffer_load_b32(from, vo, so, 0));
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int t = 0; t < 2; ++t)
+    if (t < n) v[t] = __builtin_bit_cast(O, __builtin_amdgcn_raw_buffer_load_b16(from, vo + 2 * t, so, 0));
+  return v;
+}
+template <class O, bool FULL>
+__device__ __forceinline__ void narrow_store(typename Vec<O, 2>::V v, rsrc_t to, int vo, int so, int n) {
+  if (FULL) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, v), to, vo, so, 0);
+  } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * i + r;  // and 4 q, which vo and rows hold
-      V2 o;
+    for (int t = 0; t < 2; ++t)
+      if (t < n) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (O)v[t]), to, vo + 2 * t, so, 0);
+  }
+}
+// One row's 2 features (whose sums hold the biases): h, or dg and du `du` bytes on, with their column sums; n features
+// are there, nz of them (with the padding of [dg | du]) are written
+template <class O, int EPI, int ACT, bool FULL>
+__device__ __forceinline__ void narrow_row(const float (&g)[2], const float (&u)[2], typename Vec<O, 2>::V d, rsrc_t to,
+                                           int vo, int so, int du, int n, int nz, float (&cg)[2], float (&cu)[2]) {
+  typename Vec<O, 2>::V o, p;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) o[t] = (O)(act_value<true, ACT>(acc[0][t][i][r]) * acc[1][t][i][r]);
-      if (FULL) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, o), out, vo, row * pitch, 0);
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (row < rows && t < n)
-            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (O)o[t]), out, vo + 2 * t, row * pitch, 0);
-      }
+  for (int t = 0; t < 2; ++t) {
+    if (EPI == EPI_FWD) {
+      o[t] = (O)(act_value<true, ACT>(g[t]) * u[t]);
+    } else {
+      float v;
+      const float da = act_grad<true, ACT>(g[t], v), dt = (float)d[t];
+      const float og = FULL || t < n ? dt * u[t] * da : 0.0f, ou = FULL || t < n ? dt * v : 0.0f;
+      cg[t] += og;
+      cu[t] += ou;
+      o[t] = (O)og;
+      p[t] = (O)ou;
     }
+  }
+  narrow_store<O, FULL>(o, to, vo, so, EPI == EPI_FWD ? n : nz);
+  if (EPI == EPI_BWD) narrow_store<O, FULL>(p, to, vo, so + du, nz);
 }
 
-template <class E, class O, int ACT, int KS>
+template <class E, class O, int EPI, int ACT, int KS>
 __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   constexpr int ES = elem_size<E>(), kNarrowRows = narrow_rows_of(KS * 64), TM = kNarrowRows / 16, TNH = 2;
   constexpr int IM = KS / 2, SG = kNarrowF / 32;
   constexpr bool PIPED = KS == 8;
+  static_assert(EPI == EPI_FWD || PIPED, "the backward's: wider than 128");
   __shared__ __attribute__((aligned(1024))) char lds_w[IM * 2 * kNarrowF * kRowB];
   __shared__ float lds_b[2][kNarrowF];                                   // biases
   // tiles_n blocks of features x tiles_m groups of rows; an XCD's work-groups share row groups
@@ -819,8 +840,17 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   // runs beside the other's products
   const bool ahead = wave < 4;
   i32x4 x[TM][KS];
+  typedef typename Vec<O, 2>::V V2;
+  constexpr int NP = TM * 4;  // a lane's rows of a tile
+  float cg[SG][TNH], cu[SG][TNH];  // column sums of the wave's rows, by group of features
+#pragma unroll
+  for (int i = 0; i < SG; ++i)
+#pragma unroll
+    for (int t = 0; t < TNH; ++t) cg[i][t] = cu[i][t] = 0.0f;
   // 4-byte accesses of pairs of features: all 128 there, and rows on 4-byte boundaries
-  const bool whole = n0 + kNarrowF <= g.N && (g.N & 1) == 0 && ((uintptr_t)g.out[0] & 3) == 0;
+  const bool whole = n0 + kNarrowF <= g.N && (g.N & 1) == 0 &&
+                     (((uintptr_t)g.out[0] | (EPI == EPI_BWD ? (uintptr_t)g.dh : 0)) & 3) == 0;
+  const int pitch = (int)g.ldo * 2, pd = g.N * 2, du = (int)g.fpad * 2;
   const int step = g.tiles_m * 8, tiles = (int)((g.M + kNarrowRows - 1) / kNarrowRows);
   int tile = wave * g.tiles_m + rg;
   auto tile_rsrc = [&](int t) {
@@ -844,20 +874,16 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 
   // A whole tile: a group's outputs are made between the products of the next one, a few instructions behind
   // each, so that the matrix unit and the others work at the same time in every wave.
-  auto piped = [&](rsrc_t ro, rsrc_t rn) {
+  auto piped = [&](rsrc_t ro, rsrc_t rd, rsrc_t rn) {
     if constexpr (PIPED) {
-    typedef typename Vec<O, 2>::V V2;
-    constexpr int NP = TM * 4;  // pieces of a group's epilogue: 2 features of a row
-    const int pitch = (int)g.ldo * 2;
     f32x4 acc[2][2][TNH][TM];
+    V2 d[2][EPI == EPI_BWD ? NP : 1];
     auto piece = [&](int sgi, int p) {
-      const int i = p / 4, row = 16 * i + p % 4;
-      V2 o;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        o[t] = (O)(act_value<true, ACT>(acc[sgi & 1][0][t][i][p % 4]) * acc[sgi & 1][1][t][i][p % 4]);
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, o), ro, 4 * q * pitch + (n0 + sgi * 32 + l * TNH) * 2,
-                                            row * pitch, 0);
+      const int i = p / 4, e = p % 4;
+      const float gv[2] = {acc[sgi & 1][0][0][i][e], acc[sgi & 1][0][1][i][e]};
+      const float uv[2] = {acc[sgi & 1][1][0][i][e], acc[sgi & 1][1][1][i][e]};
+      narrow_row<O, EPI, ACT, true>(gv, uv, d[sgi & 1][EPI == EPI_BWD ? p : 0], ro, 4 * q * pitch + (n0 + sgi * 32 + l * TNH) * 2,
+                                    (16 * i + e) * pitch, du, 2, 2, cg[sgi], cu[sgi]);
     };
 #pragma unroll
     for (int sgi = 0; sgi < SG; ++sgi) {
@@ -877,6 +903,12 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 #pragma unroll
           for (int i = 0; i < TM; ++i) acc[sgi & 1][h][t][i] = f32x4{v, v, v, v};
         }
+      if (EPI == EPI_BWD) {  // dh of this group, used beside the next one's products
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          d[sgi & 1][EPI == EPI_BWD ? p : 0] =
+              narrow_load<O, true>(rd, 4 * q * pd + (n0 + sgi * 32 + l * TNH) * 2, (16 * (p / 4) + p % 4) * pd, 2);
+      }
       read(0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -899,7 +931,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 #pragma unroll
         for (int n = 0; n < 4 * TM; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                        // an MFMA,
-          __builtin_amdgcn_sched_group_barrier(0x002, ACT == ACT_GELU ? 6 : 3, 0);  // what runs beside it
+          __builtin_amdgcn_sched_group_barrier(0x002, (ACT == ACT_GELU ? 6 : 3) * (EPI == EPI_BWD ? 2 : 1), 0);  // what runs beside it
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -912,6 +944,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   for (; tile < tiles; tile += step) {
     const int64_t mt = (int64_t)tile * kNarrowRows;
     const rsrc_t ro = make_rsrc(static_cast<char*>(g.out[0]) + mt * g.ldo * 2, 0x7fffffff);
+    const rsrc_t rd = make_rsrc(static_cast<const char*>(g.dh) + mt * g.N * 2, 0x7fffffff);
     const bool full = whole && mt + kNarrowRows <= g.M;
     const rsrc_t rn = tile_rsrc(tile + step);
     auto group = [&](int sgi, auto last) {
@@ -925,6 +958,17 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
           const float v = lds_b[h][c + t];
           c0[h][t] = f32x4{v, v, v, v};
         }
+      const int rows = (int)(g.M - mt < kNarrowRows ? g.M - mt : kNarrowRows) - 4 * q, f = n0 + c, n = g.N - f;
+      V2 d[EPI == EPI_BWD ? NP : 1];
+      if (EPI == EPI_BWD) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int row = 16 * (p / 4) + p % 4, vd = 4 * q * pd + f * 2;
+          V2& v = d[EPI == EPI_BWD ? p : 0];
+          if (!PIPED && full) v = narrow_load<O, true>(rd, vd, row * pd, 2);
+          else v = narrow_load<O, false>(rd, vd, row * pd, row < rows ? n : 0);
+        }
+      }
       const PCST_LDS char* ws = w + sgi * 32 * kRowB;
       i32x4 b[2][2][TNH];
       auto read = [&](int ks) {
@@ -953,19 +997,46 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      const int pitch = (int)g.ldo * 2, vo = 4 * q * pitch + (n0 + c) * 2;
-      const int rows = (int)(g.M - mt < kNarrowRows ? g.M - mt : kNarrowRows) - 4 * q;
-      if (!PIPED && full)
-        narrow_rows<O, ACT, true>(acc, ro, vo, pitch, rows, 2);
-      else
-        narrow_rows<O, ACT, false>(acc, ro, vo, pitch, rows, g.N - n0 - c);
+      // (rows past the end: nothing is written, and dh's zeros add nothing to the column sums)
+      auto rows_out = [&](auto whole_rows) {
+        constexpr bool FULL = decltype(whole_rows)::value;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int i = p / 4, row = 16 * i + p % 4;
+          const float gv[2] = {acc[0][0][i][p % 4], acc[0][1][i][p % 4]}, uv[2] = {acc[1][0][i][p % 4], acc[1][1][i][p % 4]};
+          if (FULL || row < rows)
+            narrow_row<O, EPI, ACT, FULL>(gv, uv, d[EPI == EPI_BWD ? p : 0], ro, 4 * q * pitch + f * 2, row * pitch, du, n,
+                                          (int)g.fpad - f, cg[sgi], cu[sgi]);
+        }
+      };
+      if (!PIPED && full) rows_out(std::true_type{});
+      else rows_out(std::false_type{});
     };
     if (PIPED && full) {
-      piped(ro, rn);
+      piped(ro, rd, rn);
       continue;
     }
+#pragma unroll
     for (int sgi = 0; sgi < SG - 1; ++sgi) group(sgi, std::false_type{});
     group(SG - 1, std::true_type{});
+  }
+  if (EPI == EPI_BWD && g.bpart) {
+    float* bp = g.bpart + ((int64_t)rg * 8 + wave) * 2 * g.N + n0;
+#pragma unroll
+    for (int sgi = 0; sgi < SG; ++sgi)
+#pragma unroll
+      for (int t = 0; t < TNH; ++t) {
+        float a = cg[sgi][t], b = cu[sgi][t];
+        a += __shfl_xor(a, 16, 64);
+        a += __shfl_xor(a, 32, 64);
+        b += __shfl_xor(b, 16, 64);
+        b += __shfl_xor(b, 32, 64);
+        const int c = sgi * 32 + l * TNH + t;
+        if (q == 0 && n0 + c < g.N) {
+          bp[c] = a;
+          bp[g.N + c] = b;
+        }
+      }
   }
 }
 
@@ -1037,14 +1108,16 @@ inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bo
   return best;
 }
 inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
-// narrow rows (16-bit forward): taken where 5 us and 1.13 (k of 256 bytes: 1.57) for each tile of a CU, as measured
-// (us; 60000 x 512: D = 128 28 against 40 for the tiles above, 256 42 against 55), are less than the tiles' estimate
+// narrow rows (16 bits): taken where 5 us and 1.13 (k of 256 bytes: 1.57) for each tile of a CU, as measured (us;
+// forward of 60000 x 512: D = 128 28 against 40 for the tiles above, 256 42 against 55), are less than the tiles'
+// estimate.  The backward's form the same from 129 features on (60000 x 256 x 512: 62 against 84, 30000 rows 42 against
+// 44; at 128 no gain).
 inline int64_t narrow_groups(int64_t M, int64_t F, int64_t kbytes) {
   return std::max<int64_t>(1, std::min<int64_t>(256 / cdiv(F, kNarrowF), cdiv(cdiv(M, narrow_rows_of(kbytes)), 8)));
 }
-inline bool take_narrow(int64_t M, int64_t D, int64_t F) {
+inline bool take_narrow(int64_t M, int64_t D, int64_t F, bool bwd) {
   const int64_t kbytes = 2 * D;
-  if (kbytes > kNarrowBytes || cdiv(F, kNarrowF) > 256) return false;
+  if (kbytes > kNarrowBytes || cdiv(F, kNarrowF) > 256 || (bwd && kbytes <= 256)) return false;
   const int64_t each = cdiv(cdiv(M, narrow_rows_of(kbytes)), narrow_groups(M, F, kbytes));
   return 5.0 + (kbytes <= 256 ? 1.57 : 1.13) * (double)each < plan_gated(M, D, F, 2).us;
 }
@@ -1075,7 +1148,8 @@ inline int64_t part_floats(int64_t M, int64_t D, int64_t F, int es, bool bwd) {
 // rows of bias partials: one for each wave's rows of a tile, or for 16 rows where k is split (few rows a
 // work-group: the splits' values are fetched one row after the other)
 constexpr int kFinishRows = 16;
-inline int64_t bias_parts(int64_t M, const Plan& p) {
+inline int64_t bias_parts(int64_t M, int64_t D, int64_t F, int es, const Plan& p) {
+  if (es == 2 && take_narrow(M, D, F, true)) return 8 * narrow_groups(M, F, D * es);  // its waves' rows
   return p.splits > 1 ? cdiv(M, kFinishRows) : cdiv(M, kTilings[p.tiling].bm) * kTilings[p.tiling].wm;
 }
 
@@ -1106,17 +1180,21 @@ int launch(GemmArgs& g, int tiling, hipStream_t s) {
   if (tiling == 0 && EPI != EPI_RAW) return launch_tiling<E, O, NMN, MMN, EPI, ACT, EPI == EPI_RAW ? 1 : 0>(g, s);
   return tiling == 1 ? launch_tiling<E, O, NMN, MMN, EPI, ACT, 1>(g, s) : launch_tiling<E, O, NMN, MMN, EPI, ACT, 2>(g, s);
 }
-template <class E, class O, int ACT>
+template <class E, class O, int EPI, int ACT>
 int launch_narrow(GemmArgs& g, hipStream_t s) {
   g.tiles_n = (int)cdiv(g.N, kNarrowF);
   g.tiles_m = (int)narrow_groups(g.M, g.N, g.K * elem_size<E>());
   g.ntiles = g.tiles_n * g.tiles_m;
   g.per_xcd = (int)cdiv(g.ntiles, 8);
   const dim3 grid((unsigned)(g.per_xcd * 8));
-  if (g.K * elem_size<E>() <= 256)
-    hipLaunchKernelGGL((narrow_kernel<E, O, ACT, 4>), grid, dim3(512), 0, s, g);
-  else
-    hipLaunchKernelGGL((narrow_kernel<E, O, ACT, 8>), grid, dim3(512), 0, s, g);
+  if constexpr (EPI == EPI_FWD) {
+    if (g.K * elem_size<E>() <= 256) {
+      hipLaunchKernelGGL((narrow_kernel<E, O, EPI, ACT, 4>), grid, dim3(512), 0, s, g);
+      PCST_LAUNCH_CHECK("gated_linear");
+      return PCST_OK;
+    }
+  }
+  hipLaunchKernelGGL((narrow_kernel<E, O, EPI, ACT, 8>), grid, dim3(512), 0, s, g);
   PCST_LAUNCH_CHECK("gated_linear");
   return PCST_OK;
 }
@@ -1230,6 +1308,12 @@ int launch_finish(const FinishArgs& a, int act, hipStream_t s) {
 // the forward (EPI_FWD, into out) or the recomputing backward (EPI_BWD, into [dg | du])
 template <class E, class O, int EPI>
 int run_gated(GemmArgs& g, const Plan& p, int act, float* part, hipStream_t s) {
+  if constexpr (elem_size<E>() == 2) {
+    if (take_narrow(g.M, g.K, g.N, EPI == EPI_BWD))
+      return act == ACT_SILU   ? launch_narrow<E, O, EPI, ACT_SILU>(g, s)
+             : act == ACT_GELU ? launch_narrow<E, O, EPI, ACT_GELU>(g, s)
+                               : launch_narrow<E, O, EPI, ACT_RELU>(g, s);
+  }
   if (p.splits == 1) return launch_act<E, O, EPI>(g, p.tiling, act, s);
   const FinishArgs a{part,  p.splits, g.M, g.N, g.bg, g.bu, g.bias_f32, g.xs, g.gs, g.us, g.dh, g.out[0], g.ldo, g.fpad,
                      g.bpart};
@@ -1282,12 +1366,6 @@ int fwd_out(const FwdCall& c, hipStream_t s) {
     return c.act == ACT_SILU   ? launch_rows<E, O, ACT_SILU>(g, s)
            : c.act == ACT_GELU ? launch_rows<E, O, ACT_GELU>(g, s)
                                : launch_rows<E, O, ACT_RELU>(g, s);
-  if constexpr (elem_size<E>() == 2) {
-    if (take_narrow(c.M, c.D, c.F))
-      return c.act == ACT_SILU   ? launch_narrow<E, O, ACT_SILU>(g, s)
-             : c.act == ACT_GELU ? launch_narrow<E, O, ACT_GELU>(g, s)
-                                 : launch_narrow<E, O, ACT_RELU>(g, s);
-  }
   return run_gated<E, O, EPI_FWD>(g, plan_gated(c.M, c.D, c.F, elem_size<E>()), c.act, c.part, s);
 }
 
@@ -1381,7 +1459,7 @@ int bwd_impl(const BwdCall& c, hipStream_t s) {
   const Plan pg = plan_gated(f.M, f.D, f.F, ES);
   int rc = run_gated<E, T, EPI_BWD>(g, pg, f.act, f.part, s);
   if (rc) return rc;
-  BiasArgs bias{g.bpart, (int)f.F, (int)bias_parts(f.M, pg), c.bgrad_f32, c.dbg, c.dbu};
+  BiasArgs bias{g.bpart, (int)f.F, (int)bias_parts(f.M, f.D, f.F, ES, pg), c.bgrad_f32, c.dbg, c.dbu};
   const Plan pw = plan_dw(f.M, f.D, f.F, ES);
   const Plan px = plan_dx(f.M, f.D, f.F, ES);
   const bool with_dx = c.dx && px.splits > 1, with_dw = !with_dx && (c.dwg || c.dwu) && pw.splits > 1;

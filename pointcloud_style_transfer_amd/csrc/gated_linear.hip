@@ -54,7 +54,7 @@ Layout lay(void* ws, int dt, int64_t M, int64_t D, int64_t F, bool pad, bool bwd
   l.fpad = cdiv(F, 64) * 64;
   if (bwd) {
     l.dgu = c.take<char>((size_t)(M * 2 * l.fpad * es));
-    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, gated::plan_gated(M, D, F, es)) * 2 * F));
+    l.bpart = c.take<float>((size_t)(gated::bias_parts(M, D, F, es, gated::plan_gated(M, D, F, es)) * 2 * F));
   }
   l.part = c.take<float>((size_t)gated::part_floats(M, D, F, es, bwd));
   l.bytes = c.bytes();

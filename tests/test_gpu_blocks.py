@@ -353,6 +353,26 @@ def test_gated_few_rows(M, D, F, dtype):
         bw.fill_(math.nan)
 
 
+# the backward of many rows of 129 to 256 columns (the weights stay in LDS): rows and columns that end inside a tile,
+# odd sizes, column sums of each wave's rows
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("M,D,F", [(30000, 200, 301), (24577, 130, 640), (20001, 256, 512), (17000, 255, 385), (40000, 136, 1000)])
+def test_gated_narrow_backward(M, D, F, dtype):
+    act, bt = ["silu", "gelu", "relu"][F % 3], F32 if D % 4 else dtype
+    x, k = rand(1, M, D, dtype=dtype), D ** -0.5
+    wg, wu = rand(2, F, D, dtype=dtype, scale=k), rand(3, F, D, dtype=dtype, scale=k)
+    dh, bg, bu = rand(6, M, F, dtype=dtype), rand(4, F, dtype=bt), rand(5, F, dtype=bt)
+    grads = _hip.gated_linear_bwd(x, wg, wu, dh, bg, bu, act)
+    check_grads(x, wg, wu, bg, bu, act, dh, grads, dtype)
+    for a, b in zip(grads, _hip.gated_linear_bwd(x, wg, wu, dh, bg, bu, act)):
+        assert torch.equal(a, b)
+    shifted = torch.empty(dh.numel() + 1, device="cuda", dtype=dtype)[1:].view_as(dh).copy_(dh)
+    for a, b in zip(grads[:3], _hip.gated_linear_bwd(x, wg, wu, shifted, bg, bu, act)):
+        assert torch.equal(a, b)
+    bare = _hip.gated_linear_bwd(x, wg, wu, dh, act=act)
+    check_grads(x, wg, wu, None, None, act, dh, bare, dtype)
+
+
 # few tiles and a long k, which is split: in h (long D), in dx (long F), in dW (many rows)
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("M,D,F", [(65, 4000, 70), (100, 2999, 301), (300, 2000, 40), (70, 1000, 33), (5000, 65, 701),
