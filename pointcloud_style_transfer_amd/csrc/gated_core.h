@@ -803,8 +803,8 @@ template <class E, class O, int EPI, int ACT, int KS>
 __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   constexpr int ES = elem_size<E>(), kNarrowRows = narrow_rows_of(KS * 64), TM = kNarrowRows / 16, TNH = 2;
   constexpr int IM = KS / 2, SG = kNarrowF / 32;
-  constexpr bool PIPED = KS == 8;
-  static_assert(EPI == EPI_FWD || PIPED, "the backward's: wider than 128");
+  constexpr bool PIPED = KS == 8 && EPI == EPI_FWD;
+  static_assert(KS == 8 || EPI == EPI_FWD, "the backward's: wider than 128");
   __shared__ __attribute__((aligned(1024))) char lds_w[IM * 2 * kNarrowF * kRowB];
   __shared__ float lds_b[2][kNarrowF];                                   // biases
   // tiles_n blocks of features x tiles_m groups of rows; an XCD's work-groups share row groups
@@ -847,10 +847,14 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
   for (int i = 0; i < SG; ++i)
 #pragma unroll
     for (int t = 0; t < TNH; ++t) cg[i][t] = cu[i][t] = 0.0f;
-  // 4-byte accesses of pairs of features: all 128 there, and rows on 4-byte boundaries
-  const bool whole = n0 + kNarrowF <= g.N && (g.N & 1) == 0 &&
-                     (((uintptr_t)g.out[0] | (EPI == EPI_BWD ? (uintptr_t)g.dh : 0)) & 3) == 0;
-  const int pitch = (int)g.ldo * 2, pd = g.N * 2, du = (int)g.fpad * 2;
+  // 4-byte accesses of pairs of features: an even number of them, rows on 4-byte boundaries; pairs past the end are
+  // sent past the buffer's (dh's are zeros there, as the sums are, and so is what is written up to fpad)
+  const bool pairs = (g.N & 1) == 0 && (((uintptr_t)g.out[0] | (EPI == EPI_BWD ? (uintptr_t)g.dh : 0)) & 3) == 0;
+  const int pitch = (int)g.ldo * 2, pd = g.N * 2, du = (int)g.fpad * 2, limit = EPI == EPI_FWD ? g.N : (int)g.fpad;
+  auto pair_at = [&](int sgi, int row, int end) {
+    const int f = n0 + sgi * 32 + l * TNH;
+    return f < end ? 4 * q * row + f * 2 : (int)0x80000000;
+  };
   const int step = g.tiles_m * 8, tiles = (int)((g.M + kNarrowRows - 1) / kNarrowRows);
   int tile = wave * g.tiles_m + rg;
   auto tile_rsrc = [&](int t) {
@@ -874,16 +878,15 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 
   // A whole tile: a group's outputs are made between the products of the next one, a few instructions behind
   // each, so that the matrix unit and the others work at the same time in every wave.
-  auto piped = [&](rsrc_t ro, rsrc_t rd, rsrc_t rn) {
+  auto piped = [&](rsrc_t ro, rsrc_t rn) {
     if constexpr (PIPED) {
     f32x4 acc[2][2][TNH][TM];
-    V2 d[2][EPI == EPI_BWD ? NP : 1];
     auto piece = [&](int sgi, int p) {
       const int i = p / 4, e = p % 4;
       const float gv[2] = {acc[sgi & 1][0][0][i][e], acc[sgi & 1][0][1][i][e]};
       const float uv[2] = {acc[sgi & 1][1][0][i][e], acc[sgi & 1][1][1][i][e]};
-      narrow_row<O, EPI, ACT, true>(gv, uv, d[sgi & 1][EPI == EPI_BWD ? p : 0], ro, 4 * q * pitch + (n0 + sgi * 32 + l * TNH) * 2,
-                                    (16 * i + e) * pitch, du, 2, 2, cg[sgi], cu[sgi]);
+      narrow_row<O, EPI, ACT, true>(gv, uv, V2{}, ro, pair_at(sgi, pitch, limit), (16 * i + e) * pitch, du, 2, 2, cg[sgi],
+                                    cu[sgi]);
     };
 #pragma unroll
     for (int sgi = 0; sgi < SG; ++sgi) {
@@ -903,12 +906,6 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 #pragma unroll
           for (int i = 0; i < TM; ++i) acc[sgi & 1][h][t][i] = f32x4{v, v, v, v};
         }
-      if (EPI == EPI_BWD) {  // dh of this group, used beside the next one's products
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          d[sgi & 1][EPI == EPI_BWD ? p : 0] =
-              narrow_load<O, true>(rd, 4 * q * pd + (n0 + sgi * 32 + l * TNH) * 2, (16 * (p / 4) + p % 4) * pd, 2);
-      }
       read(0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -931,7 +928,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
 #pragma unroll
         for (int n = 0; n < 4 * TM; ++n) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                        // an MFMA,
-          __builtin_amdgcn_sched_group_barrier(0x002, (ACT == ACT_GELU ? 6 : 3) * (EPI == EPI_BWD ? 2 : 1), 0);  // what runs beside it
+          __builtin_amdgcn_sched_group_barrier(0x002, ACT == ACT_GELU ? 6 : 3, 0);  // what runs beside it
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -945,7 +942,7 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
     const int64_t mt = (int64_t)tile * kNarrowRows;
     const rsrc_t ro = make_rsrc(static_cast<char*>(g.out[0]) + mt * g.ldo * 2, 0x7fffffff);
     const rsrc_t rd = make_rsrc(static_cast<const char*>(g.dh) + mt * g.N * 2, 0x7fffffff);
-    const bool full = whole && mt + kNarrowRows <= g.M;
+    const bool full = pairs && mt + kNarrowRows <= g.M;
     const rsrc_t rn = tile_rsrc(tile + step);
     auto group = [&](int sgi, auto last) {
       // the sums start at the biases
@@ -963,10 +960,10 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
       if (EPI == EPI_BWD) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          const int row = 16 * (p / 4) + p % 4, vd = 4 * q * pd + f * 2;
+          const int row = 16 * (p / 4) + p % 4;
           V2& v = d[EPI == EPI_BWD ? p : 0];
-          if (!PIPED && full) v = narrow_load<O, true>(rd, vd, row * pd, 2);
-          else v = narrow_load<O, false>(rd, vd, row * pd, row < rows ? n : 0);
+          if (full) v = narrow_load<O, true>(rd, pair_at(sgi, pd, g.N), row * pd, 2);
+          else v = narrow_load<O, false>(rd, 4 * q * pd + f * 2, row * pd, row < rows ? n : 0);
         }
       }
       const PCST_LDS char* ws = w + sgi * 32 * kRowB;
@@ -1005,15 +1002,16 @@ __global__ __launch_bounds__(512, 2) void narrow_kernel(GemmArgs g) {
           const int i = p / 4, row = 16 * i + p % 4;
           const float gv[2] = {acc[0][0][i][p % 4], acc[0][1][i][p % 4]}, uv[2] = {acc[1][0][i][p % 4], acc[1][1][i][p % 4]};
           if (FULL || row < rows)
-            narrow_row<O, EPI, ACT, FULL>(gv, uv, d[EPI == EPI_BWD ? p : 0], ro, 4 * q * pitch + f * 2, row * pitch, du, n,
-                                          (int)g.fpad - f, cg[sgi], cu[sgi]);
+            narrow_row<O, EPI, ACT, FULL>(gv, uv, d[EPI == EPI_BWD ? p : 0], ro,
+                                          FULL ? pair_at(sgi, pitch, limit) : 4 * q * pitch + f * 2, row * pitch, du, n,
+                                          limit - f, cg[sgi], cu[sgi]);
         }
       };
       if (!PIPED && full) rows_out(std::true_type{});
       else rows_out(std::false_type{});
     };
     if (PIPED && full) {
-      piped(ro, rd, rn);
+      piped(ro, rn);
       continue;
     }
 #pragma unroll
@@ -1110,8 +1108,8 @@ inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bo
 inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
 // narrow rows (16 bits): taken where 5 us and 1.13 (k of 256 bytes: 1.57) for each tile of a CU, as measured (us;
 // forward of 60000 x 512: D = 128 28 against 40 for the tiles above, 256 42 against 55), are less than the tiles'
-// estimate.  The backward's form the same from 129 features on (60000 x 256 x 512: 62 against 84, 30000 rows 42 against
-// 44; at 128 no gain).
+// estimate.  The backward's form the same from 129 columns on (a pass with its gradients, 60000 x 256 x 512: 207 against
+// 217, 120000 rows 396 against 432, 30000 the same; at 128 columns no gain).
 inline int64_t narrow_groups(int64_t M, int64_t F, int64_t kbytes) {
   return std::max<int64_t>(1, std::min<int64_t>(256 / cdiv(F, kNarrowF), cdiv(cdiv(M, narrow_rows_of(kbytes)), 8)));
 }
