@@ -1108,8 +1108,9 @@ inline Plan plan(int64_t rows, int64_t cols, int64_t K, int segs, int groups, bo
 inline Plan plan_gated(int64_t M, int64_t D, int64_t F, int es) { return plan(M, F, D, 1, 1, false, es, 2 * M * F); }
 // narrow rows (16 bits): taken where 5 us and 1.13 (k of 256 bytes: 1.57) for each tile of a CU, as measured (us;
 // forward of 60000 x 512: D = 128 28 against 40 for the tiles above, 256 42 against 55), are less than the tiles'
-// estimate.  The backward's form the same from 129 columns on (a pass with its gradients, 60000 x 256 x 512: 207 against
-// 217, 120000 rows 396 against 432, 30000 the same; at 128 columns no gain).
+// estimate.  The backward's form waits for dh and x longer, and both write twice as much: 20 us and 1.93 for each
+// tile against 1.7 times the estimate (x 256 x 512 out of HBM: 30000 rows 49 against 46, 60000 76 against 88, 120000
+// 134 against 180); up to 128 columns no gain.
 inline int64_t narrow_groups(int64_t M, int64_t F, int64_t kbytes) {
   return std::max<int64_t>(1, std::min<int64_t>(256 / cdiv(F, kNarrowF), cdiv(cdiv(M, narrow_rows_of(kbytes)), 8)));
 }
@@ -1117,7 +1118,8 @@ inline bool take_narrow(int64_t M, int64_t D, int64_t F, bool bwd) {
   const int64_t kbytes = 2 * D;
   if (kbytes > kNarrowBytes || cdiv(F, kNarrowF) > 256 || (bwd && kbytes <= 256)) return false;
   const int64_t each = cdiv(cdiv(M, narrow_rows_of(kbytes)), narrow_groups(M, F, kbytes));
-  return 5.0 + (kbytes <= 256 ? 1.57 : 1.13) * (double)each < plan_gated(M, D, F, 2).us;
+  const double tiles = plan_gated(M, D, F, 2).us;
+  return bwd ? 20.0 + 1.93 * (double)each < 1.7 * tiles : 5.0 + (kbytes <= 256 ? 1.57 : 1.13) * (double)each < tiles;
 }
 // few rows: always up to 16 (no workspace to ask for), up to 128 where 3.5 us and 0.45 + 0.19 for each 16 rows of x
 // per 512 bytes of k and 256 work-groups are less than the tiles' estimate, the launch that adds their splits
