@@ -58,7 +58,8 @@ def quant_rows(x):
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up), x [..., D], weights [F, D] -> [..., F], in one
     kernel.  Operands of one type (float32, bfloat16 or float16; under torch.autocast they are rounded
-    to its type), biases of that type or float32; act "silu", "gelu" or "relu".  Differentiable."""
+    to its type), biases of that type or float32; act "silu", "gelu" or "relu".  Differentiable; relu's gradient
+    may fall on either side where the gate is within the rounding of its own sum (1e-6 of the terms) of zero."""
     if (x.dim() != 2 or torch.is_autocast_enabled("cuda") or _wants_grad(x, w_gate, w_up, b_gate, b_up)):
         return _ag.GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, act)
     return _hip.gated_linear(x, w_gate, w_up, b_gate, b_up, act)
